@@ -12,6 +12,10 @@ from .abi import (  # noqa: F401
     TIER_OZAKI1,
     TIER_OZAKI2_FAST,
     TIER_DGEMM,
+    DTYPE_F64,
+    DTYPE_F32,
+    DTYPE_F16,
+    DTYPE_BF16,
     load_library,
     library_path,
 )
@@ -24,6 +28,10 @@ from .api import (  # noqa: F401
     conv2d,
     gemm_device,
     conv2d_device,
+    layernorm_device,
+    layernorm_gradients_device,
+    token_logprobs_device,
+    token_logprobs_gradient_device,
     sync_status,
     stream_handle,
     launch_count,

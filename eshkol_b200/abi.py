@@ -17,6 +17,12 @@ TIER_OZAKI1 = 1
 TIER_OZAKI2_FAST = 2
 TIER_DGEMM = 3
 
+# storage types of the training and serving operators (EshkolB200Dtype)
+DTYPE_F64 = 0
+DTYPE_F32 = 1
+DTYPE_F16 = 2
+DTYPE_BF16 = 3
+
 c_double_p = ctypes.POINTER(ctypes.c_double)
 
 
@@ -151,6 +157,10 @@ def load_library() -> ctypes.CDLL:
     sig("eshkol_b200_normalize_f64_device", ctypes.c_int, [vp, vp, u64, u64, ctypes.c_double, ctypes.c_double, ctypes.c_double])
     sig("eshkol_b200_batchnorm_backward_f64_device", ctypes.c_int, [vp] * 8 + [u64, u64])
     sig("eshkol_b200_layernorm_backward_f64_device", ctypes.c_int, [vp] * 6 + [u64, u64])
+    sig("eshkol_b200_layernorm_forward_device", ctypes.c_int, [vp] * 6 + [u64] * 4 + [ctypes.c_double, ctypes.c_int])
+    sig("eshkol_b200_layernorm_gradients_device", ctypes.c_int, [vp] * 8 + [u64] * 5 + [ctypes.c_int])
+    sig("eshkol_b200_token_logprobs_device", ctypes.c_int, [vp] * 7 + [u64] * 4 + [ctypes.c_int])
+    sig("eshkol_b200_token_logprobs_gradient_device", ctypes.c_int, [vp] * 7 + [u64] * 4 + [ctypes.c_int])
     sig("eshkol_b200_sync_status", ctypes.c_int, [])
     sig("eshkol_b200_set_pair_gemm", None, [ctypes.c_int])
     sig("eshkol_b200_set_sm_limit", None, [ctypes.c_int])

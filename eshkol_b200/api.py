@@ -132,6 +132,52 @@ def conv2d_device(d_in: int, shape_in, d_ker: int, shape_ker, stride: int, pad: 
         raise RuntimeError(f"eshkol_b200_conv2d_f64_device failed ({rc})")
 
 
+def _active():
+    """The library with its device selected; raises when there is none."""
+    lib = load_library()
+    if not lib.eshkol_b200_stream() and lib.eshkol_b200_init(_current_device()) != 0:
+        raise RuntimeError("eshkol_b200_init failed: no usable sm_100 device")
+    return lib
+
+
+def layernorm_device(d_x: int, d_gamma: int, d_beta: int, d_y: int, d_mean: int, d_inv_std: int, samples: int,
+                     features: int, epsilon: float, dtype: int, ldx: int = 0, ldy: int = 0) -> None:
+    """Layer normalisation with weight vectors through eshkol_b200_layernorm_forward_device, on raw
+    device pointers (asynchronous on the library's stream; 0 for an absent array)."""
+    if _active().eshkol_b200_layernorm_forward_device(d_x, d_gamma, d_beta, d_y, d_mean, d_inv_std, samples, features,
+                                                      ldx, ldy, epsilon, dtype) != 0:
+        raise RuntimeError("eshkol_b200_layernorm_forward_device failed")
+
+
+def layernorm_gradients_device(d_grad_out: int, d_x: int, d_mean: int, d_inv_std: int, d_gamma: int, d_grad_in: int,
+                               d_grad_gamma: int, d_grad_beta: int, samples: int, features: int, dtype: int,
+                               ld_grad_out: int = 0, ldx: int = 0, ld_grad_in: int = 0) -> None:
+    """grad_in, grad_gamma and grad_beta of layernorm_device from its saved statistics."""
+    if _active().eshkol_b200_layernorm_gradients_device(d_grad_out, d_x, d_mean, d_inv_std, d_gamma, d_grad_in,
+                                                        d_grad_gamma, d_grad_beta, samples, features, ld_grad_out, ldx,
+                                                        ld_grad_in, dtype) != 0:
+        raise RuntimeError("eshkol_b200_layernorm_gradients_device failed")
+
+
+def token_logprobs_device(d_logits: int, d_tokens: int, d_logprob: int, d_entropy: int, d_lse: int, d_top_logprob: int,
+                          d_top_index: int, rows: int, vocab: int, n_top: int, dtype: int, ld: int = 0) -> None:
+    """Log probabilities of given tokens, entropy, log of the sum and top alternatives of rows of logits
+    through eshkol_b200_token_logprobs_device (asynchronous; 0 for an output that is not wanted)."""
+    if _active().eshkol_b200_token_logprobs_device(d_logits, d_tokens, d_logprob, d_entropy, d_lse, d_top_logprob,
+                                                   d_top_index, rows, vocab, ld, n_top, dtype) != 0:
+        raise RuntimeError("eshkol_b200_token_logprobs_device failed")
+
+
+def token_logprobs_gradient_device(d_logits: int, d_tokens: int, d_lse: int, d_entropy: int, d_grad_logprob: int,
+                                   d_grad_entropy: int, d_grad_logits: int, rows: int, vocab: int, dtype: int,
+                                   ld: int = 0, ld_grad: int = 0) -> None:
+    """Gradient of the logits from the gradients of logprob and entropy (either may be 0)."""
+    if _active().eshkol_b200_token_logprobs_gradient_device(d_logits, d_tokens, d_lse, d_entropy, d_grad_logprob,
+                                                            d_grad_entropy, d_grad_logits, rows, vocab, ld, ld_grad,
+                                                            dtype) != 0:
+        raise RuntimeError("eshkol_b200_token_logprobs_gradient_device failed")
+
+
 _device = None
 
 

@@ -15,6 +15,7 @@
 #include <mutex>
 #include <vector>
 
+#include "b200_elem.cuh"
 #include "b200_internal.h"
 #include "b200_ozaki2.h"
 #include "b200_tiers.h"
@@ -1208,6 +1209,7 @@ void eshkol_b200_shutdown(void) {
   if (!g.ready) return;
   cudaStreamSynchronize(g.stream);
   staged_shutdown();
+  op_scratch_shutdown();
   if (g.ws) cudaFree(g.ws);
   if (g.aux) cudaFree(g.aux);
   if (g.tbuf) cudaFree(g.tbuf);

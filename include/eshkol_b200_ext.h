@@ -285,6 +285,65 @@ int eshkol_b200_layernorm_backward_f64_device(const double* grad_out, const doub
                                               const double* saved_gamma, double* grad_input, uint64_t samples,
                                               uint64_t features);
 
+/* ---- operators of language-model training and serving on tensors stored in f64, f32, f16 or bf16 ----
+ * No counterpart in the reference, whose tensors are f64.  Device pointers; asynchronous on the library
+ * stream, whatever device is current; 0, or -1 on bad arguments or a failed launch.  A pitch ("ld...") is
+ * the distance of a matrix's rows in elements, 0 for dense rows; bases and pitches need only the alignment
+ * of their element type (multiples of 16 bytes are read and written in 16-byte words).  Elements between
+ * the rows of a result are left as they were.  Zero samples or rows are a valid call that computes
+ * nothing (sums over them are zero).  Statistics and the gradients of vectors are f64 for f64 tensors and
+ * f32 otherwise ("stat type"); sums are held in that type and combined in a fixed order, so equal calls
+ * give equal bits.  Arrays must not overlap unless the call says so.
+ * Scratch belongs to the library and is ordered by its stream.  Calls captured from that stream into a
+ * CUDA graph get scratch of the graph's own, so graphs may be replayed on any stream and beside eager
+ * calls; a replay itself is ordered by the stream it is launched on. */
+typedef enum {
+  ESHKOL_B200_F64 = 0,
+  ESHKOL_B200_F32 = 1,
+  ESHKOL_B200_F16 = 2,
+  ESHKOL_B200_BF16 = 3
+} EshkolB200Dtype;
+
+/* Layer normalisation with weight vectors: with mean and inv_std = 1 / sqrt(population variance +
+ * epsilon) of a sample's features,
+ *   y = (x - mean) * inv_std * gamma + beta.
+ * x, y [samples x features] and gamma, beta [features] in `dtype`; gamma or beta may be NULL (1, 0).
+ * mean, inv_std [samples] in the stat type, each may be NULL.  y may be x with the same pitch. */
+int eshkol_b200_layernorm_forward_device(const void* x, const void* gamma, const void* beta, void* y,
+                                         void* mean, void* inv_std, uint64_t samples, uint64_t features,
+                                         uint64_t ldx, uint64_t ldy, double epsilon, int dtype);
+/* Its gradients from the saved mean and inv_std: grad_in [samples x features] in `dtype`; grad_gamma,
+ * grad_beta [features] in the stat type, each may be NULL, as may gamma.  grad_in may be grad_out with the
+ * same pitch. */
+int eshkol_b200_layernorm_gradients_device(const void* grad_out, const void* x, const void* mean,
+                                           const void* inv_std, const void* gamma, void* grad_in,
+                                           void* grad_gamma, void* grad_beta, uint64_t samples,
+                                           uint64_t features, uint64_t ld_grad_out, uint64_t ldx,
+                                           uint64_t ld_grad_in, int dtype);
+
+/* Log probabilities of given tokens under rows of logits [rows x vocab], vocab <= 2^30, rows <= 2^24:
+ *   lse = log sum exp(logits),  logprob = logits[token] - lse,  entropy = -sum p log p
+ * and the n_top <= 32 largest logits of every row: their log probabilities [rows x n_top] and indices,
+ * largest first, equal logits by index.  tokens [rows]; a negative token stands for a position without
+ * one (logprob 0), a token >= vocab gives NaN.  logprob, entropy, lse, top_logprob are in the stat type;
+ * each output may be NULL, not all of them; n_top is 0 exactly when both top outputs are NULL; tokens may
+ * be NULL when logprob is.  Entries of minus infinity are masked: probability 0.  A row of nothing else has lse and
+ * logprob minus infinity and entropy 0.  A row with NaN or plus infinity has NaN outputs; its
+ * alternatives are those of its numbers, with index -1 where there are too few. */
+int eshkol_b200_token_logprobs_device(const void* logits, const int64_t* tokens, void* logprob,
+                                      void* entropy, void* lse, void* top_logprob, int64_t* top_index,
+                                      uint64_t rows, uint64_t vocab, uint64_t ld, uint64_t n_top, int dtype);
+/* Gradient with respect to the logits from the saved lse and entropy, with p = exp(logits - lse):
+ *   grad_logits[j] = grad_logprob * ([j = token] - p[j]) - grad_entropy * p[j] * (log p[j] + entropy)
+ * grad_logprob or grad_entropy (stat type, [rows]) may be NULL, not both; entropy may be NULL without
+ * grad_entropy, tokens without grad_logprob.  Positions without a token get no gradient from
+ * grad_logprob; a token >= vocab makes its row NaN; a row without unmasked entries gets zeros.
+ * grad_logits may be logits with the same pitch. */
+int eshkol_b200_token_logprobs_gradient_device(const void* logits, const int64_t* tokens, const void* lse,
+                                               const void* entropy, const void* grad_logprob,
+                                               const void* grad_entropy, void* grad_logits, uint64_t rows,
+                                               uint64_t vocab, uint64_t ld, uint64_t ld_grad, int dtype);
+
 /* Waits for the stream, then returns 0 if every kernel since the previous call
  * completed normally, a positive kernel status code if a bounded wait inside a
  * kernel ran out, or -1 on a CUDA error. */

@@ -79,3 +79,72 @@ def layernorm_backward(grad_out, x, mean, inv_std, gamma):
     sum_g = g.sum(axis=1, keepdims=True)
     sum_gn = (g * nz).sum(axis=1, keepdims=True)
     return (inv_std[:, None] / D) * (D * g - sum_g - nz * sum_gn)
+
+
+# ---- training and serving operators, in f64 from their definitions (no counterpart in the reference)
+def layernorm_forward(x, gamma, beta, eps):
+    """(y, mean, inv_std) of layer normalisation with weight vectors."""
+    x = np.asarray(x, dtype=np.float64)
+    mean = x.mean(axis=1)
+    inv_std = 1.0 / np.sqrt(((x - mean[:, None]) ** 2).mean(axis=1) + eps)
+    y = (x - mean[:, None]) * inv_std[:, None]
+    return y * (1.0 if gamma is None else gamma) + (0.0 if beta is None else beta), mean, inv_std
+
+
+def layernorm_gradients(g, x, mean, inv_std, gamma):
+    """(grad_in, grad_gamma, grad_beta) from saved statistics."""
+    xhat = (x - mean[:, None]) * inv_std[:, None]
+    u = g * (1.0 if gamma is None else gamma)
+    n = x.shape[1]
+    grad_in = inv_std[:, None] * (u - u.sum(axis=1, keepdims=True) / n - xhat * (u * xhat).sum(axis=1, keepdims=True) / n)
+    return grad_in, (g * xhat).sum(axis=0), g.sum(axis=0)
+
+
+def token_logprobs(x, tokens, n_top):
+    """(logprob, entropy, lse, top_logprob, top_index): masked entries are minus infinity, a negative
+    token stands for none, equal logits go by index.  A row with NaN or plus infinity is NaN and its
+    alternatives are those of its numbers (index -1 where there are too few)."""
+    x = np.asarray(x, dtype=np.float64)
+    rows, vocab = x.shape
+    bad = (np.isnan(x) | (x == np.inf)).any(axis=1)
+    with np.errstate(all="ignore"):
+        m = np.where(np.isnan(x), -np.inf, x).max(axis=1)
+        m0 = np.where(np.isfinite(m), m, 0.0)[:, None]
+        e = np.where(np.isnan(x), 0.0, np.exp(np.where(x == np.inf, 0.0, x - m0)))
+        s = e.sum(axis=1)
+        lse = np.where(bad, np.nan, m0[:, 0] + np.log(s))
+        d = np.where(e > 0, x - m0, 0.0)
+        ent = np.where(bad, np.nan, np.where(s > 0, np.log(s) - (e * d).sum(axis=1) / np.where(s > 0, s, 1.0), 0.0))
+
+        def log_prob(v, l):
+            return np.where(np.isnan(l), np.nan, np.where(v == -np.inf, -np.inf, v - l))
+
+        logprob = np.zeros(rows)
+        for r in range(rows):
+            if tokens[r] >= vocab:
+                logprob[r] = np.nan
+            elif tokens[r] >= 0:
+                logprob[r] = log_prob(x[r, tokens[r]], lse[r])
+        top_lp, top_i = np.full((rows, n_top), np.nan), np.full((rows, n_top), -1, dtype=np.int64)
+        for r in range(rows):
+            order = np.argsort(np.where(np.isnan(x[r]), np.inf, -x[r]), kind="stable")
+            order = order[~np.isnan(x[r][order])][:n_top]
+            top_i[r, :len(order)] = order
+            top_lp[r, :len(order)] = log_prob(x[r][order], lse[r])
+    return logprob, ent, lse, top_lp, top_i
+
+
+def token_logprobs_gradient(x, tokens, lse, entropy, g, h):
+    """Gradient of the logits; g, h: gradients of logprob and entropy."""
+    x = np.asarray(x, dtype=np.float64)
+    with np.errstate(all="ignore"):
+        lp = x - lse[:, None]
+        p = np.where(lse[:, None] == -np.inf, 0.0, np.exp(lp))
+        g = np.where(tokens >= 0, g, 0.0)
+        grad = -p * g[:, None] - h[:, None] * np.where(p > 0, p * (lp + entropy[:, None]), 0.0)
+    for r in range(x.shape[0]):
+        if tokens[r] >= x.shape[1]:
+            grad[r] = np.nan
+        elif tokens[r] >= 0:
+            grad[r, tokens[r]] += g[r]
+    return grad
