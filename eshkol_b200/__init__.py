@@ -8,6 +8,7 @@ row-sharded multi-GPU driver built on ``torch.distributed``.
 from .abi import (  # noqa: F401
     EshkolGPUBuffer,
     GemmOpts,
+    LinearOpts,
     TIER_OZAKI2,
     TIER_OZAKI1,
     TIER_OZAKI2_FAST,
@@ -30,6 +31,9 @@ from .api import (  # noqa: F401
     conv2d_device,
     layernorm_device,
     layernorm_gradients_device,
+    make_linear_opts,
+    linear_device,
+    linear_gradients_device,
     token_logprobs_device,
     token_logprobs_gradient_device,
     sync_status,

@@ -66,6 +66,23 @@ class GemmOpts(ctypes.Structure):
     ]
 
 
+class LinearOpts(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("trans_w", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("pre", ctypes.c_void_p),
+        ("ldx", ctypes.c_int64),
+        ("ldw", ctypes.c_int64),
+        ("ldy", ctypes.c_int64),
+        ("ld_residual", ctypes.c_int64),
+        ("ld_pre", ctypes.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -159,6 +176,9 @@ def load_library() -> ctypes.CDLL:
     sig("eshkol_b200_layernorm_backward_f64_device", ctypes.c_int, [vp] * 6 + [u64, u64])
     sig("eshkol_b200_layernorm_forward_device", ctypes.c_int, [vp] * 6 + [u64] * 4 + [ctypes.c_double, ctypes.c_int])
     sig("eshkol_b200_layernorm_gradients_device", ctypes.c_int, [vp] * 8 + [u64] * 5 + [ctypes.c_int])
+    lop = ctypes.POINTER(LinearOpts)
+    sig("eshkol_b200_linear_forward_device", ctypes.c_int, [vp] * 3 + [u64] * 3 + [lop])
+    sig("eshkol_b200_linear_gradients_device", ctypes.c_int, [vp] * 6 + [u64] * 3 + [lop])
     sig("eshkol_b200_token_logprobs_device", ctypes.c_int, [vp] * 7 + [u64] * 4 + [ctypes.c_int])
     sig("eshkol_b200_token_logprobs_gradient_device", ctypes.c_int, [vp] * 7 + [u64] * 4 + [ctypes.c_int])
     sig("eshkol_b200_sync_status", ctypes.c_int, [])

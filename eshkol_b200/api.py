@@ -11,7 +11,7 @@ import ctypes
 
 import numpy as np
 
-from .abi import GemmOpts, load_library
+from .abi import GemmOpts, LinearOpts, load_library
 
 _MODULI = (256, 255, 253, 251, 247, 241, 239, 233, 229, 227, 223, 217, 211, 199, 197, 193)
 
@@ -157,6 +157,27 @@ def layernorm_gradients_device(d_grad_out: int, d_x: int, d_mean: int, d_inv_std
                                                         d_grad_gamma, d_grad_beta, samples, features, ld_grad_out, ldx,
                                                         ld_grad_in, dtype) != 0:
         raise RuntimeError("eshkol_b200_layernorm_gradients_device failed")
+
+
+def make_linear_opts(dtype: int, activation: int = 0, trans_w: bool = False, bias: int = 0, residual: int = 0, pre: int = 0,
+                     ldx: int = 0, ldw: int = 0, ldy: int = 0, ld_residual: int = 0, ld_pre: int = 0) -> LinearOpts:
+    """Options of linear_device and linear_gradients_device (device pointers, 0 for an absent array)."""
+    return LinearOpts(dtype, activation, 1 if trans_w else 0, 0, bias or None, residual or None, pre or None, ldx, ldw, ldy,
+                      ld_residual, ld_pre)
+
+
+def linear_device(d_x: int, d_w: int, d_y: int, rows: int, d_in: int, d_out: int, opts: LinearOpts) -> None:
+    """y = activation(x w + bias) + residual through eshkol_b200_linear_forward_device (asynchronous)."""
+    if _active().eshkol_b200_linear_forward_device(d_x, d_w, d_y, rows, d_in, d_out, ctypes.byref(opts)) != 0:
+        raise RuntimeError("eshkol_b200_linear_forward_device failed")
+
+
+def linear_gradients_device(d_grad_out: int, d_x: int, d_w: int, d_grad_x: int, d_grad_w: int, d_grad_bias: int,
+                            rows: int, d_in: int, d_out: int, opts: LinearOpts) -> None:
+    """grad_x, grad_w and grad_bias (0 for one that is not wanted) of linear_device."""
+    if _active().eshkol_b200_linear_gradients_device(d_grad_out, d_x, d_w, d_grad_x, d_grad_w, d_grad_bias, rows, d_in,
+                                                     d_out, ctypes.byref(opts)) != 0:
+        raise RuntimeError("eshkol_b200_linear_gradients_device failed")
 
 
 def token_logprobs_device(d_logits: int, d_tokens: int, d_logprob: int, d_entropy: int, d_lse: int, d_top_logprob: int,

@@ -240,6 +240,24 @@ int make_plane_map(CUtensorMap* map, const void* base, long long inner_bytes, lo
   return 0;
 }
 
+int make_matrix_map16(CUtensorMap* map, const void* base, long long inner, long long rows, long long ld,
+                      long long planes, long long plane_stride, int box_rows) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(plane_stride) * 2};
+  const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_rows), 1u};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  const CUresult r = g.encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box,
+                              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    fprintf(stderr, "[eshkol-b200] cuTensorMapEncodeTiled failed (%d): inner=%lld rows=%lld ld=%lld\n",
+            static_cast<int>(r), inner, rows, ld);
+    return -1;
+  }
+  return 0;
+}
+
 static void fill_mod_job(GemmJob* j, int a_plane, int b_plane, int out_plane, unsigned p) {
   memset(j, 0, sizeof(*j));
   j->n_seg = 1;
@@ -1197,6 +1215,7 @@ int eshkol_b200_init(int device) {
   }
   B200_CHECK(split_set_attributes());
   B200_CHECK(tiers_set_attributes());
+  B200_CHECK(linear_set_attributes());
   // the allocation-free entry point's scratch array: its module is loaded and its address
   // resolved here, so that entry point itself never causes a load or an allocation
   if (static_scratch_setup(device) != 0) return -1;

@@ -20,6 +20,10 @@ int* lib_status_word();
 void count_launches(int n);
 int make_plane_map(CUtensorMap* map, const void* base, long long inner_bytes, long long rows,
                    long long planes, long long plane_stride, int box_rows);
+// a row-major matrix of 16-bit elements (`inner` in a row, pitch `ld`), `planes` of them plane_stride
+// elements apart, tiled {64 elements, box_rows, 1} with the 128-byte swizzle; zero beyond its extent
+int make_matrix_map16(CUtensorMap* map, const void* base, long long inner, long long rows, long long ld,
+                      long long planes, long long plane_stride, int box_rows);
 void oz2_host_consts(int n_mod, Oz2DeviceConsts* c, double* log2P);
 int ozaki2_exact_gemm_im2col(const double* dA, const Im2colView& view, double* dC, long long M, long long K,
                              long long N, const EshkolB200GemmOpts& o);
@@ -44,6 +48,7 @@ int f16_gemm(const double* dA, const double* dB, double* dC, long long batch, lo
              long long N);
 int f32_gemm(const float* dA, const float* dB, float* dC, long long M, long long K, long long N);
 cudaError_t tiers_set_attributes();
+cudaError_t linear_set_attributes();  // b200_linear.cu
 // b200_static_scratch.cu: resolve the fixed scratch array's address on `device` (current)
 int static_scratch_setup(int device);
 // dst[cols x rows] = transpose of src[rows x cols] (row-major f64)

@@ -321,6 +321,34 @@ int eshkol_b200_layernorm_gradients_device(const void* grad_out, const void* x, 
                                            uint64_t features, uint64_t ld_grad_out, uint64_t ldx,
                                            uint64_t ld_grad_in, int dtype);
 
+/* Linear layer of f32, f16 and bf16 tensors: with z = x w + bias,
+ *   y = activation(z) + residual
+ * x [rows x d_in], w [d_in x d_out] (with trans_w [d_out x d_in]), bias [d_out], residual, y and pre
+ * [rows x d_out], all in opts->dtype.  16-bit operands are multiplied on the tensor cores as they lie
+ * (rows that are not on 16-byte boundaries are copied to scratch first) with f32 sums; f32 operands as
+ * three bf16 parts each, exact to f32 rounding for finite values below 3.38e38 (others give NaN).  f64
+ * tensors are refused: eshkol_b200_gemm_f64_device and _feed_forward_f64_device serve them. */
+typedef struct EshkolB200LinearOpts {
+  int32_t dtype;            /* EshkolB200Dtype: F32, F16 or BF16 */
+  int32_t activation;       /* 0 none, 1 ReLU, 2 tanh-form GELU, as in EshkolB200GemmOpts */
+  int32_t trans_w;          /* 1: w is stored d_out x d_in */
+  int32_t reserved;
+  const void* bias;         /* or NULL */
+  const void* residual;     /* or NULL; may be y with the same pitch */
+  void* pre;                /* forward: z goes here as well, or NULL; gradients: z as saved (with an activation) */
+  int64_t ldx, ldw, ldy, ld_residual, ld_pre; /* pitches, 0 for dense rows */
+} EshkolB200LinearOpts;
+int eshkol_b200_linear_forward_device(const void* x, const void* w, void* y, uint64_t rows, uint64_t d_in,
+                                      uint64_t d_out, const EshkolB200LinearOpts* opts);
+/* Its gradients: with dz = grad_out * activation'(pre), rounded to the storage type for the products,
+ *   grad_x = dz w^T,  grad_w = x^T dz (stored as w is),  grad_bias = column sums of the unrounded dz
+ * grad_out [rows x d_out] has the pitch ldy, grad_x that of x, grad_w that of w; grad_bias [d_out] is f32.
+ * Each result may be NULL, not all of them; x may be NULL without grad_w, w without grad_x.  opts->bias
+ * and residual are not read (the residual's gradient is grad_out).  No result may overlap an input. */
+int eshkol_b200_linear_gradients_device(const void* grad_out, const void* x, const void* w, void* grad_x,
+                                        void* grad_w, void* grad_bias, uint64_t rows, uint64_t d_in,
+                                        uint64_t d_out, const EshkolB200LinearOpts* opts);
+
 /* Log probabilities of given tokens under rows of logits [rows x vocab], vocab <= 2^30, rows <= 2^24:
  *   lse = log sum exp(logits),  logprob = logits[token] - lse,  entropy = -sum p log p
  * and the n_top <= 32 largest logits of every row: their log probabilities [rows x n_top] and indices,

@@ -148,3 +148,36 @@ def token_logprobs_gradient(x, tokens, lse, entropy, g, h):
         elif tokens[r] >= 0:
             grad[r, tokens[r]] += g[r]
     return grad
+
+
+GELU_A, GELU_B = np.sqrt(2.0 / np.pi), 0.044715
+
+
+def activate(z, act):
+    """0 none, 1 ReLU, 2 the tanh form of GELU."""
+    if act == 1:
+        return np.where(z > 0, z, 0.0)
+    if act == 2:
+        return 0.5 * z * (1.0 + np.tanh(GELU_A * (z + GELU_B * z ** 3)))
+    return z
+
+
+def activate_slope(z, act):
+    if act == 1:
+        return (z > 0).astype(np.float64)
+    if act == 2:
+        t = np.tanh(GELU_A * (z + GELU_B * z ** 3))
+        return 0.5 * (1.0 + t) + 0.5 * z * (1.0 - t * t) * GELU_A * (1.0 + 3.0 * GELU_B * z ** 2)
+    return np.ones_like(z)
+
+
+def linear_forward(x, w, bias, residual, act):
+    """(y, pre) of the linear layer, w [d_in x d_out]."""
+    z = x @ w + (0.0 if bias is None else bias)
+    return activate(z, act) + (0.0 if residual is None else residual), z
+
+
+def linear_gradients(g, x, w, pre, act):
+    """(grad_x, grad_w, grad_bias, dz)."""
+    dz = g * activate_slope(pre, act) if act else g
+    return dz @ w.T, x.T @ dz, dz.sum(axis=0), dz

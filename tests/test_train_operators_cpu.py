@@ -76,3 +76,34 @@ def test_token_logprob_gradient_against_differences():
     want = differences(loss, x)
     x[1, 3] = keep
     assert np.abs(got - want).max() < NEAR
+
+
+@pytest.mark.parametrize("act", [0, 1, 2])
+def test_linear_gradients_against_differences(act):
+    x, w, g = inputs.normal(81, (4, 6)), inputs.normal(82, (6, 5)), inputs.normal(83, (4, 5))
+    bias = inputs.normal(84, (5,))
+
+    def loss():
+        return float((g * ref.linear_forward(x, w, bias, None, act)[0]).sum())
+
+    pre = ref.linear_forward(x, w, bias, None, act)[1]
+    assert np.abs(pre).min() > 1e-4  # no difference crosses ReLU's corner
+    gx, gw, gb, _ = ref.linear_gradients(g, x, w, pre, act)
+    assert np.abs(gx - differences(loss, x)).max() < 10 * NEAR
+    assert np.abs(gw - differences(loss, w)).max() < 10 * NEAR
+    assert np.abs(gb - differences(loss, bias)).max() < 10 * NEAR
+
+
+def test_linear_calls_are_refused_without_a_device():
+    lib = eb.load_library()
+    if lib.eshkol_gpu_init() == 1:
+        pytest.skip("a GPU is present")
+    a, out = np.ones((4, 4), dtype=np.float32), np.full((4, 4), 7.0, dtype=np.float32)
+    p, o = a.ctypes.data, out.ctypes.data
+    opts = eb.make_linear_opts(eb.DTYPE_F32)
+    assert ctypes.sizeof(opts) == 80
+    assert lib.eshkol_b200_linear_forward_device(p, p, o, 4, 4, 4, ctypes.byref(opts)) == -1
+    assert lib.eshkol_b200_linear_gradients_device(p, p, p, o, o, o, 4, 4, 4, ctypes.byref(opts)) == -1
+    assert (out == 7.0).all()
+    with pytest.raises(RuntimeError):
+        eb.linear_device(p, p, o, 4, 4, 4, opts)
