@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace b200 {
 
 template <typename T> struct Elem;
@@ -38,13 +40,136 @@ template <typename T, int kV> struct alignas(sizeof(T) * kV) Pack {
 
 template <typename T> constexpr int kVec16 = 16 / static_cast<int>(sizeof(T));
 
+// ------------------------------------------------------------------ two values at a time
+// f32 pairs go through the packed f32x2 instructions (one issue slot for two additions, products or fused
+// multiply-adds, each rounded as its scalar form); f64 pairs are two scalars.
+template <typename A> struct Duo;
+template <> struct Duo<float> {
+  unsigned long long v;
+  static __device__ __forceinline__ Duo of(float x, float y) {
+    Duo r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+    return r;
+  }
+  __device__ __forceinline__ float lo() const {
+    float x;
+    asm("mov.b64 {%0, _}, %1;" : "=f"(x) : "l"(v));
+    return x;
+  }
+  __device__ __forceinline__ float hi() const {
+    float y;
+    asm("mov.b64 {_, %0}, %1;" : "=f"(y) : "l"(v));
+    return y;
+  }
+};
+template <> struct Duo<double> {
+  double x, y;
+  static __device__ __forceinline__ Duo of(double a, double b) { return Duo{a, b}; }
+  __device__ __forceinline__ double lo() const { return x; }
+  __device__ __forceinline__ double hi() const { return y; }
+};
+template <typename A> __device__ __forceinline__ Duo<A> both(A x) { return Duo<A>::of(x, x); }
+__device__ __forceinline__ Duo<float> operator+(Duo<float> a, Duo<float> b) {
+  Duo<float> r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Duo<float> operator*(Duo<float> a, Duo<float> b) {
+  Duo<float> r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Duo<float> fma2(Duo<float> a, Duo<float> b, Duo<float> c) {
+  Duo<float> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Duo<double> operator+(Duo<double> a, Duo<double> b) { return {a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ Duo<double> operator*(Duo<double> a, Duo<double> b) { return {a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ Duo<double> fma2(Duo<double> a, Duo<double> b, Duo<double> c) {
+  return {fma(a.x, b.x, c.x), fma(a.y, b.y, c.y)};
+}
+template <typename A> __device__ __forceinline__ A total(Duo<A> a) { return a.lo() + a.hi(); }
+
+// sixteen bytes as pairs in the stat type, and back with one rounding
+template <typename T> using Word = Pack<T, kVec16<T>>;
+template <typename T> constexpr int kDuos = kVec16<T> / 2;
+__device__ __forceinline__ void widen_word(const Word<double>& p, Duo<double> (&d)[1]) { d[0] = {p.v[0], p.v[1]}; }
+__device__ __forceinline__ void widen_word(const Word<float>& p, Duo<float> (&d)[2]) {
+  d[0] = Duo<float>::of(p.v[0], p.v[1]);
+  d[1] = Duo<float>::of(p.v[2], p.v[3]);
+}
+__device__ __forceinline__ void widen_word(const Word<__half>& p, Duo<float> (&d)[4]) {
+  const __half2* h = reinterpret_cast<const __half2*>(&p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    d[i] = Duo<float>::of(f.x, f.y);
+  }
+}
+__device__ __forceinline__ void widen_word(const Word<__nv_bfloat16>& p, Duo<float> (&d)[4]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(&p);  // a bf16 is the upper half of its f32
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = Duo<float>::of(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+}
+__device__ __forceinline__ Word<double> narrow_word(const Duo<double> (&d)[1]) {
+  Word<double> p;
+  p.v[0] = d[0].x; p.v[1] = d[0].y;
+  return p;
+}
+__device__ __forceinline__ Word<float> narrow_word(const Duo<float> (&d)[2]) {
+  Word<float> p;
+  p.v[0] = d[0].lo(); p.v[1] = d[0].hi(); p.v[2] = d[1].lo(); p.v[3] = d[1].hi();
+  return p;
+}
+template <typename T> __device__ __forceinline__ Word<T> narrow_word(const Duo<float> (&d)[4]) {
+  Word<T> p;
+  if constexpr (sizeof(T) == 2) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(d[i].hi()), "f"(d[i].lo()));
+      else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(d[i].hi()), "f"(d[i].lo()));
+    }
+  }
+  return p;
+}
+template <typename T, int kD> __device__ __forceinline__ Word<T> to_word(const Duo<typename Elem<T>::Acc> (&d)[kD]) {
+  if constexpr (sizeof(T) == 2) return narrow_word<T>(d);
+  else return narrow_word(d);
+}
+
+// Sixteen bytes' worth of a row of n elements from element c: one word where `words` says that the row's
+// words are aligned and it lies whole in the row, else element by element, `otherwise` outside.
+template <typename T> __device__ __forceinline__ Word<T> read_word(const T* row, int c, int n, bool words, T otherwise) {
+  constexpr int kV = kVec16<T>;
+  if (words && c + kV <= n) return *reinterpret_cast<const Word<T>*>(row + c);
+  Word<T> p;
+#pragma unroll
+  for (int j = 0; j < kV; ++j) p.v[j] = c + j < n ? row[c + j] : otherwise;
+  return p;
+}
+template <typename T> __device__ __forceinline__ void write_word(T* row, int c, int n, bool words, const Word<T>& p) {
+  constexpr int kV = kVec16<T>;
+  if (words && c + kV <= n) {
+    *reinterpret_cast<Word<T>*>(row + c) = p;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < kV; ++j)
+    if (c + j < n) row[c + j] = p.v[j];
+}
+
 // elements between p and the 16-byte boundary at or before it
 template <typename T> __host__ __device__ __forceinline__ int elems_past_boundary(const T* p) {
   return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
 }
 
-__device__ __forceinline__ float sum_rsqrt(float v) { return 1.0f / sqrtf(v); }
-__device__ __forceinline__ double sum_rsqrt(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ float inverse_root(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double inverse_root(double v) { return rsqrt(v); }
 
 // every lane gets the sum over the warp (the same tree on every lane)
 template <typename A> __device__ __forceinline__ A warp_sum(A v) {
@@ -53,19 +178,78 @@ template <typename A> __device__ __forceinline__ A warp_sum(A v) {
   return v;
 }
 
-// every thread of the block gets both sums; sm holds 2 * 32 values and may be reused after the
-// next barrier
-template <typename A> __device__ __forceinline__ void block_sum2(A& a, A& b, A* sm, int warps) {
+// Every thread of the block gets the sum, or both sums.  sm (32 or 64 values) may be written again by a
+// reduction that has another block-wide reduction or barrier between itself and this one: callers
+// alternate between two arrays, which leaves one barrier per reduction.
+template <typename A> __device__ __forceinline__ A block_sum(A a, A* sm, int warps) {
   a = warp_sum(a);
-  b = warp_sum(b);
-  if (warps == 1) return;
+  if (warps == 1) return a;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) sm[w] = a;
   __syncthreads();
-  if (lane == 0) { sm[w] = a; sm[32 + w] = b; }
-  __syncthreads();
-  // the partial sums are added by shuffles, the same tree in every warp
-  a = warp_sum(lane < warps ? sm[lane] : A(0));
-  b = warp_sum(lane < warps ? sm[32 + lane] : A(0));
+  return warp_sum(lane < warps ? sm[lane] : A(0));
+}
+template <typename A> __device__ __forceinline__ void block_sum2(A& a, A& b, A* sm, int warps) {
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, at = lane & 15;
+  // the lower half of the warp goes on with a, the upper half with b: half the shuffles
+  A v = (half ? b : a) + __shfl_xor_sync(0xffffffffu, half ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (warps > 1) {
+    if (at == 0) sm[half * 32 + w] = v;
+    __syncthreads();
+    v = (at < warps ? sm[half * 32 + at] : A(0)) + (at + 16 < warps ? sm[half * 32 + at + 16] : A(0));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+  a = __shfl_sync(0xffffffffu, v, 0);
+  b = __shfl_sync(0xffffffffu, v, 16);
+}
+
+// Copies from global to shared memory that a thread waits for by itself (cp.async): 16 bytes, or one
+// element of 4 or 8
+__device__ __forceinline__ void copy_async16(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(shared))), "l"(global) : "memory");
+}
+template <int kBytes> __device__ __forceinline__ void copy_async_small(void* shared, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(shared))), "l"(global), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void wait_async() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+// How a row's words get from memory to the threads that work on them, some rows ahead: in registers, or
+// through shared memory in copies of words or of elements
+enum Ahead : int { kInRegisters = 0, kByWords = 1, kByElements = 2 };
+// starts the copy of the word at element c < n of a row into this thread's place
+template <typename T, int kHow> __device__ __forceinline__ void copy_word(Word<T>* place, const T* row, int c, int n) {
+  if constexpr (kHow == kByWords) {
+    copy_async16(place, row + c);
+  } else if constexpr (sizeof(T) >= 4) {
+#pragma unroll
+    for (int j = 0; j < kVec16<T>; ++j)
+      if (c + j < n) copy_async_small<sizeof(T)>(&place->v[j], row + c + j);
+  }
+}
+// the copied word, `zero` behind the row
+template <typename T, int kHow> __device__ __forceinline__ Word<T> take_word(const Word<T>* place, int c, int n, T zero) {
+  Word<T> p;
+  if (kHow == kByWords ? c < n : c + kVec16<T> <= n) return *place;
+#pragma unroll
+  for (int j = 0; j < kVec16<T>; ++j) p.v[j] = (kHow == kByElements && c + j < n) ? place->v[j] : zero;
+  return p;
+}
+// read_word and write_word where kByWords promises that every word is aligned and whole, c < n
+template <typename T, int kHow> __device__ __forceinline__ Word<T> get_word(const T* row, int c, int n, bool words, T otherwise) {
+  if constexpr (kHow == kByWords) return *reinterpret_cast<const Word<T>*>(row + c);
+  else return read_word(row, c, n, words, otherwise);
+}
+template <typename T, int kHow> __device__ __forceinline__ void put_word(T* row, int c, int n, bool words, const Word<T>& p) {
+  if constexpr (kHow == kByWords) *reinterpret_cast<Word<T>*>(row + c) = p;
+  else write_word(row, c, n, words, p);
 }
 
 // A device pointer's alignment and a row pitch both a multiple of 16 bytes

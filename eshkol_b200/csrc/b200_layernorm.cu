@@ -13,103 +13,148 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <cooperative_groups.h>
+
 #include "b200_elem.cuh"
 #include "b200_tiers.h"
 
 namespace b200 {
 namespace {
+namespace cg = cooperative_groups;
 
-template <typename T, int kV, int kN>
-__device__ __forceinline__ void load_row(const T* row, int n, int first, int stride, Pack<T, kV> (&p)[kN]) {
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    const int c = (first + i * stride) * kV;
-    if (c + kV <= n) {
-      p[i] = *reinterpret_cast<const Pack<T, kV>*>(row + c);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kV; ++j) p[i].v[j] = (c + j < n) ? row[c + j] : Elem<T>::narrow(0);
-    }
-  }
+// The first places of a mean, at least 10 bits of it: x minus it is exact for x of few bits, so that sums of
+// such differences have no rounding that all terms share.
+__device__ __forceinline__ float leading_bits(float v) { return __uint_as_float(__float_as_uint(v) & 0xffffe000u); }
+__device__ __forceinline__ double leading_bits(double v) {
+  return __longlong_as_double(__double_as_longlong(v) & ~0x3ffffffffffll);
 }
 
-template <typename T, int kV>
-__device__ __forceinline__ void store_pack(T* row, int n, int c, const Pack<T, kV>& p) {
-  if (c + kV <= n) {
-    *reinterpret_cast<Pack<T, kV>*>(row + c) = p;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kV; ++j)
-      if (c + j < n) row[c + j] = p.v[j];
-  }
-}
-
-template <typename T, int kV>
-__device__ __forceinline__ Pack<T, kV> load_weights(const T* w, int n, int c, float otherwise) {
-  Pack<T, kV> p;
-  if (w && c + kV <= n) return *reinterpret_cast<const Pack<T, kV>*>(w + c);
-#pragma unroll
-  for (int j = 0; j < kV; ++j) p.v[j] = (w && c + j < n) ? w[c + j] : Elem<T>::narrow(otherwise);
-  return p;
-}
+struct NormArgs {
+  const void *x, *gamma, *beta;
+  void *y, *mean, *inv_std;
+  long long rows, ldx, ldy;
+  int n;
+  bool x_words, y_words, gamma_words, beta_words;  // rows on 16-byte boundaries
+  double epsilon;
+};
 
 // ------------------------------------------------------------------ forward
-// A row is shared by `width` threads (a warp, or the block), each holding kN packs of kV elements.
-template <typename T, int kV, int kN, bool kWarp>
-__global__ void __launch_bounds__(kWarp ? 256 : 1024) layernorm_kernel(
-    const T* x, const T* __restrict__ gamma, const T* __restrict__ beta, T* y,  // x and y may be the same
-    typename Elem<T>::Acc* __restrict__ mean_out, typename Elem<T>::Acc* __restrict__ inv_std_out, long long rows,
-    int n, long long ldx, long long ldy, typename Elem<T>::Acc epsilon) {
+// A row belongs to a warp, or to a block, whose threads hold kN words of 16 bytes each.  What a thread does
+// once per row (its share of the reductions, the root, addresses) is some 150 instructions, an element
+// about ten (packed f32 arithmetic), so a thread gets four words where rows are many.  The next kAhead
+// rows are on their way in shared memory: every thread copies the words that it will read itself.
+template <int kHow> constexpr int kNormAhead = kHow == kInRegisters ? 1 : 4;
+
+template <typename T, int kN, bool kWarp, int kMost, int kHow>
+__global__ void __launch_bounds__(kMost, kMost == 128 ? 6 : kMost == 256 ? 3 : 1) layernorm_kernel(const NormArgs a) {  // x and y may be the same
   using A = typename Elem<T>::Acc;
-  __shared__ A sm[64];
+  using D = Duo<A>;
+  constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kNormAhead<kHow>;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ A sm1[32], sm2[64];
   const int width = kWarp ? 32 : blockDim.x, warps = kWarp ? 1 : blockDim.x >> 5;
   const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
   const int per_block = kWarp ? blockDim.x >> 5 : 1, group = kWarp ? threadIdx.x >> 5 : 0;
-  const A inv_n = A(1) / A(n);
-  for (long long r = static_cast<long long>(blockIdx.x) * per_block + group; r < rows;
-       r += static_cast<long long>(gridDim.x) * per_block) {
-    Pack<T, kV> p[kN];
-    load_row<T, kV, kN>(x + r * ldx, n, t, width, p);
-    A sum = 0, none = 0;
+  const int n = a.n;
+  const T *gamma = static_cast<const T*>(a.gamma), *beta = static_cast<const T*>(a.beta);
+  const A inv_n = A(1) / A(n), epsilon = static_cast<A>(a.epsilon);
+  const T zero = Elem<T>::narrow(0), one = Elem<T>::narrow(1);
+  const long long first = static_cast<long long>(blockIdx.x) * per_block + group;
+  const long long step = static_cast<long long>(gridDim.x) * per_block;
+  const T* in = static_cast<const T*>(a.x) + first * a.ldx;  // the next row to come
+  T* out = static_cast<T*>(a.y) + first * a.ldy;
+  const long long in_step = step * a.ldx, out_step = step * a.ldy;
+  long long coming = first;
+  Word<T>* ring = reinterpret_cast<Word<T>*>(dyn) + threadIdx.x;  // [stage][word of the row][thread]
+  const auto fetch = [&](int stage) {
+    if constexpr (kHow != kInRegisters) {
+      if (coming < a.rows) {
 #pragma unroll
-    for (int i = 0; i < kN; ++i)
-#pragma unroll
-      for (int j = 0; j < kV; ++j) sum += Elem<T>::widen(p[i].v[j]);  // places behind the row hold zero
-    block_sum2(sum, none, sm, warps);
-    const A mean0 = sum * inv_n;
-    A ds = 0, sq = 0;
-#pragma unroll
-    for (int i = 0; i < kN; ++i)
-#pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const A d = ((t + i * width) * kV + j < n) ? Elem<T>::widen(p[i].v[j]) - mean0 : A(0);
-        ds += d;
-        sq += d * d;
+        for (int i = 0; i < kN; ++i) {
+          const int c = (t + i * width) * kV;
+          if (c < n) copy_word<T, kHow>(ring + (stage * kN + i) * blockDim.x, in, c, n);
+        }
       }
-    block_sum2(ds, sq, sm, warps);
-    // mean0 carries the rounding of a long sum; the deviations' own mean is what it is off by
-    const A off = ds * inv_n;
-    const A var = sq * inv_n - off * off;
-    const A r_std = sum_rsqrt((var > A(0) ? var : var * A(0)) + epsilon);  // a NaN stays one
-    if (t == 0) {
-      if (mean_out) mean_out[r] = mean0 + off;
-      if (inv_std_out) inv_std_out[r] = r_std;
+      commit_async();
+      coming += step;
+      in += in_step;
     }
-    T* out = y + r * ldy;
+  };
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) fetch(s);
+  int stage = 0;
+  for (long long r = first; r < a.rows; r += step) {
+    D d[kN][kD];
+    if constexpr (kHow != kInRegisters) {
+      wait_async<kAhead - 1>();
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        widen_word(take_word<T, kHow>(ring + (stage * kN + i) * blockDim.x, (t + i * width) * kV, n, zero), d[i]);
+      fetch(stage);
+      stage = stage + 1 == kAhead ? 0 : stage + 1;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) widen_word(read_word(in, (t + i * width) * kV, n, a.x_words, zero), d[i]);
+      in += in_step;
+    }
+    D sum2[kD];
+#pragma unroll
+    for (int j = 0; j < kD; ++j) sum2[j] = d[0][j];
+#pragma unroll
+    for (int i = 1; i < kN; ++i)
+#pragma unroll
+      for (int j = 0; j < kD; ++j) sum2[j] = sum2[j] + d[i][j];  // places behind the row hold zero
+#pragma unroll
+    for (int j = 1; j < kD; ++j) sum2[0] = sum2[0] + sum2[j];
+    const A pivot = leading_bits(block_sum(total(sum2[0]), sm1, warps) * inv_n);
+    D ds2[kD], sq2[kD];
+#pragma unroll
+    for (int j = 0; j < kD; ++j) ds2[j] = sq2[j] = both(A(0));
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int c = (t + i * width) * kV;
       if (c >= n) break;
-      const Pack<T, kV> g = load_weights<T, kV>(gamma, n, c, 1.f), b = load_weights<T, kV>(beta, n, c, 0.f);
-      Pack<T, kV> o;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const A xhat = ((Elem<T>::widen(p[i].v[j]) - mean0) - off) * r_std;
-        o.v[j] = Elem<T>::narrow(xhat * Elem<T>::widen(g.v[j]) + Elem<T>::widen(b.v[j]));
+      for (int j = 0; j < kD; ++j) {
+        d[i][j] = d[i][j] + both(-pivot);
+        if constexpr (kHow != kByWords)  // the row may end inside a word: what is behind it deviates by nothing
+          d[i][j] = D::of(c + 2 * j < n ? d[i][j].lo() : A(0), c + 2 * j + 1 < n ? d[i][j].hi() : A(0));
+        ds2[j] = ds2[j] + d[i][j];
+        sq2[j] = fma2(d[i][j], d[i][j], sq2[j]);
       }
-      store_pack<T, kV>(out, n, c, o);
     }
+#pragma unroll
+    for (int j = 1; j < kD; ++j) {
+      ds2[0] = ds2[0] + ds2[j];
+      sq2[0] = sq2[0] + sq2[j];
+    }
+    A ds = total(ds2[0]), sq = total(sq2[0]);
+    block_sum2(ds, sq, sm2, warps);
+    const A off = ds * inv_n;  // mean = pivot + off, and |off| is below 2^-10 of the pivot
+    const A var = sq * inv_n - off * off;
+    const A r_std = inverse_root((var > A(0) ? var : var * A(0)) + epsilon);  // a NaN stays one
+    if (t == 0) {
+      if (a.mean) static_cast<A*>(a.mean)[r] = pivot + off;
+      if (a.inv_std) static_cast<A*>(a.inv_std)[r] = r_std;
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int c = (t + i * width) * kV;
+      if (c >= n) break;
+      D g[kD], b[kD];
+      if (gamma) widen_word(get_word<T, kHow>(gamma, c, n, a.gamma_words, one), g);
+      if (beta) widen_word(get_word<T, kHow>(beta, c, n, a.beta_words, zero), b);
+#pragma unroll
+      for (int j = 0; j < kD; ++j) {
+        const D xhat = (d[i][j] + both(-off)) * both(r_std);
+        const D scaled = gamma ? xhat * g[j] : xhat;
+        d[i][j] = beta ? scaled + b[j] : scaled;
+      }
+      put_word<T, kHow>(out, c, n, a.y_words, to_word<T>(d[i]));
+    }
+    out += out_step;
   }
+  if constexpr (kHow != kInRegisters) wait_async<0>();
 }
 
 // rows longer than a block's registers hold: the row is read three times, the second and third from L2
@@ -119,16 +164,15 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(
     typename Elem<T>::Acc* __restrict__ mean_out, typename Elem<T>::Acc* __restrict__ inv_std_out, long long rows,
     int n, long long ldx, long long ldy, typename Elem<T>::Acc epsilon) {
   using A = typename Elem<T>::Acc;
-  __shared__ A sm[64];
+  __shared__ A sm1[32], sm[64];
   const int warps = blockDim.x >> 5;
   const A inv_n = A(1) / A(n);
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* in = x + r * ldx;
     T* out = y + r * ldy;
-    A sum = 0, none = 0;
+    A sum = 0;
     for (int c = threadIdx.x; c < n; c += blockDim.x) sum += Elem<T>::widen(in[c]);
-    block_sum2(sum, none, sm, warps);
-    const A mean0 = sum * inv_n;
+    const A mean0 = leading_bits(block_sum(sum, sm1, warps) * inv_n);
     A ds = 0, sq = 0;
     for (int c = threadIdx.x; c < n; c += blockDim.x) {
       const A d = Elem<T>::widen(in[c]) - mean0;
@@ -138,7 +182,7 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(
     block_sum2(ds, sq, sm, warps);
     const A off = ds * inv_n;
     const A var = sq * inv_n - off * off;
-    const A r_std = sum_rsqrt((var > A(0) ? var : var * A(0)) + epsilon);
+    const A r_std = inverse_root((var > A(0) ? var : var * A(0)) + epsilon);
     if (threadIdx.x == 0) {
       if (mean_out) mean_out[r] = mean0 + off;
       if (inv_std_out) inv_std_out[r] = r_std;
@@ -151,94 +195,196 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(
 }
 
 // ------------------------------------------------------------------ gradients
-// A row is shared by `width` threads (a warp of a block of eight, or the block); every thread keeps its
-// columns over all the rows of its group, and with them its share of grad_gamma and grad_beta in
-// registers.  A group's shares go to partial[group][2][n].
-template <typename T, int kV, int kN, bool kWarp>
-__global__ void __launch_bounds__(kWarp ? 256 : 512) layernorm_gradients_kernel(
-    const T* grad_out, const T* __restrict__ x, const typename Elem<T>::Acc* __restrict__ mean,
-    const typename Elem<T>::Acc* __restrict__ inv_std, const T* __restrict__ gamma, T* grad_in,
-    typename Elem<T>::Acc* __restrict__ partial, long long rows, int n, long long ldg, long long ldx, long long ldi) {
+struct NormGradArgs {
+  const void *grad_out, *x, *mean, *inv_std, *gamma;
+  void *grad_in, *grad_gamma, *grad_beta, *partial;
+  long long rows, ldg, ldx, ldi;
+  int n;
+  bool g_words, x_words, i_words, gamma_words;
+};
+
+// A row belongs to a warp, to a block, or to the blocks of a cluster, each with a contiguous part of the
+// columns.  A thread keeps its columns (kN words of 16 bytes) over all rows of its group, and with them
+// its share of grad_gamma and grad_beta in registers; a block's share goes to partial[group][2][n].  Many
+// elements a thread and few warps a row, because what a thread does once per row costs as much as ten elements.  The next rows are on their way in shared memory, kAhead of them (every thread
+// copies the words that it will read itself, so no barrier is involved), or, where the rows are not on
+// 16-byte boundaries, one in registers.
+// words a thread holds in a row of a block: 16 elements, or 8 of f64
+template <typename T> constexpr int kGradWords = sizeof(T) == 2 ? 2 : 4;
+template <int kN, int kHow> constexpr int kRowsAhead = kHow == kInRegisters ? 1 : 4;
+
+template <typename T, int kN, bool kWarp, int kHow>
+__global__ void __launch_bounds__(kWarp ? 128 : 256, kWarp ? 3 : 2) layernorm_gradients_kernel(const NormGradArgs a) {
   using A = typename Elem<T>::Acc;
-  __shared__ A sm[64];
+  using D = Duo<A>;
+  constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kRowsAhead<kN, kHow>;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ A sm[2][64];
+  __shared__ A of_blocks[2][2][8];  // the cluster's blocks' sums of two rows in turn
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = kWarp ? 1 : static_cast<int>(cluster.num_blocks());
+  const int part = kWarp ? 0 : static_cast<int>(cluster.block_rank());
   const int width = kWarp ? 32 : blockDim.x, warps = kWarp ? 1 : blockDim.x >> 5;
-  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
+  const int t = (kWarp ? threadIdx.x & 31 : threadIdx.x) + part * kN * width;  // word of the first pass
   const int per_block = kWarp ? blockDim.x >> 5 : 1, local = kWarp ? threadIdx.x >> 5 : 0;
-  const long long group = static_cast<long long>(blockIdx.x) * per_block + local;
-  const long long groups = static_cast<long long>(gridDim.x) * per_block;
+  const long long group = static_cast<long long>(blockIdx.x / parts) * per_block + local;
+  const long long groups = static_cast<long long>(gridDim.x / parts) * per_block;
+  const int n = a.n;
   const A inv_n = A(1) / A(n);
-  A sum_g[kN][kV], sum_gx[kN][kV];
+  const T zero = Elem<T>::narrow(0);
+  // the next row to come, and the next to go
+  const T *x = static_cast<const T*>(a.x) + group * a.ldx, *grad_out = static_cast<const T*>(a.grad_out) + group * a.ldg;
+  const A *mean = static_cast<const A*>(a.mean) + group, *inv_std = static_cast<const A*>(a.inv_std) + group;
+  T* out = static_cast<T*>(a.grad_in) + group * a.ldi;
+  const long long x_step = groups * a.ldx, g_step = groups * a.ldg, i_step = groups * a.ldi;
+  long long coming = group;
+  D sum_g[kN][kD], sum_gx[kN][kD];
+  Word<T> w[kN];
 #pragma unroll
-  for (int i = 0; i < kN; ++i)
+  for (int i = 0; i < kN; ++i) {
+    w[i] = read_word(static_cast<const T*>(a.gamma), (t + i * width) * kV, a.gamma ? n : 0, a.gamma_words, Elem<T>::narrow(1));
 #pragma unroll
-    for (int j = 0; j < kV; ++j) sum_g[i][j] = sum_gx[i][j] = A(0);
-  Pack<T, kV> w[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) w[i] = load_weights<T, kV>(gamma, n, (t + i * width) * kV, 1.f);
-  Pack<T, kV> px[kN], pg[kN];
-  A mu = 0, rs = 0;
-  if (group < rows) {
-    load_row<T, kV, kN>(x + group * ldx, n, t, width, px);
-    load_row<T, kV, kN>(grad_out + group * ldg, n, t, width, pg);
-    mu = mean[group];
-    rs = inv_std[group];
+    for (int j = 0; j < kD; ++j) sum_g[i][j] = sum_gx[i][j] = both(A(0));
   }
-  for (long long r = group; r < rows; r += groups) {
-    Pack<T, kV> cx[kN], cg[kN];
+  Word<T>* ring = reinterpret_cast<Word<T>*>(dyn);  // [stage][x or grad_out][word of the pass][thread]
+  const auto place = [&](int stage, int which, int i) {
+    return ring + ((stage * 2 + which) * kN + i) * blockDim.x + threadIdx.x;
+  };
+  Word<T> px[kN], pg[kN];
+  A next_m[kAhead], next_s[kAhead];
+  const auto fetch = [&](int stage) {  // stage is a constant wherever this is inlined
+    if (coming < a.rows) {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) { cx[i] = px[i]; cg[i] = pg[i]; }
-    const A m = mu, s = rs;
-    const long long next = r + groups;  // the next row is on its way while this one is worked on
-    if (next < rows) {
-      load_row<T, kV, kN>(x + next * ldx, n, t, width, px);
-      load_row<T, kV, kN>(grad_out + next * ldg, n, t, width, pg);
-      mu = mean[next];
-      rs = inv_std[next];
+      for (int i = 0; i < kN; ++i) {
+        const int c = (t + i * width) * kV;
+        if constexpr (kHow != kInRegisters) {
+          if (c < n) {
+            copy_word<T, kHow>(place(stage, 0, i), x, c, n);
+            copy_word<T, kHow>(place(stage, 1, i), grad_out, c, n);
+          }
+        } else {
+          px[i] = read_word(x, c, n, a.x_words, zero);
+          pg[i] = read_word(grad_out, c, n, a.g_words, zero);
+        }
+      }
+      next_m[stage] = *mean;
+      next_s[stage] = *inv_std;
+      x += x_step;
+      grad_out += g_step;
+      mean += groups;
+      inv_std += groups;
+      coming += groups;
     }
-    A su = 0, sux = 0;
+    if constexpr (kHow != kInRegisters) commit_async();
+  };
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) fetch(s);
+  int turn = 0;
+  if (!kWarp && parts > 1) cluster.sync();  // every block has started before any writes to another
+  for (long long r0 = group; r0 < a.rows; r0 += kAhead * groups) {
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const long long r = r0 + s * groups;
+      if (r >= a.rows) break;  // the same for the whole group
+      if constexpr (kHow != kInRegisters) wait_async<kAhead - 1>();
+      const A m = next_m[s], rs = next_s[s];
+      D xhat[kN][kD], u[kN][kD];
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int c = (t + i * width) * kV;
+        Word<T> cx, cg_;
+        if constexpr (kHow != kInRegisters) {
+          cx = take_word<T, kHow>(place(s, 0, i), c, n, zero);
+          cg_ = take_word<T, kHow>(place(s, 1, i), c, n, zero);
+        } else {
+          cx = px[i];
+          cg_ = pg[i];
+        }
+        widen_word(cx, xhat[i]);
+        widen_word(cg_, u[i]);
+      }
+      fetch(s);
+      D su2 = both(A(0)), sux2 = both(A(0));
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        D wi[kD];
+        widen_word(w[i], wi);
+#pragma unroll
+        for (int j = 0; j < kD; ++j) {  // behind the row grad_out is zero and nothing is added
+          xhat[i][j] = (xhat[i][j] + both(-m)) * both(rs);
+          sum_g[i][j] = sum_g[i][j] + u[i][j];
+          sum_gx[i][j] = fma2(u[i][j], xhat[i][j], sum_gx[i][j]);
+          u[i][j] = u[i][j] * wi[j];
+          su2 = su2 + u[i][j];
+          sux2 = fma2(u[i][j], xhat[i][j], sux2);
+        }
+      }
+      A su = total(su2), sux = total(sux2);
+      block_sum2(su, sux, sm[turn], warps);
+      if (!kWarp && parts > 1) {
+        // every block writes its sums into all blocks of the cluster; two places in turn, because a
+        // block may be one row ahead of another, but no more
+        if (threadIdx.x < parts) {
+          *cluster.map_shared_rank(&of_blocks[turn][0][part], threadIdx.x) = su;
+          *cluster.map_shared_rank(&of_blocks[turn][1][part], threadIdx.x) = sux;
+        }
+        cluster.sync();
+        su = sux = A(0);
+        for (int b = 0; b < parts; ++b) {
+          su += of_blocks[turn][0][b];
+          sux += of_blocks[turn][1][b];
+        }
+      }
+      turn ^= 1;
+      const D level = both(-su * inv_n * rs), along = both(-sux * inv_n);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int c = (t + i * width) * kV;
+        if (c >= n) break;
+#pragma unroll
+        for (int j = 0; j < kD; ++j) u[i][j] = fma2(fma2(xhat[i][j], along, u[i][j]), both(rs), level);
+        put_word<T, kHow>(out, c, n, a.i_words, to_word<T>(u[i]));
+      }
+      out += i_step;
+    }
+  }
+  if constexpr (kHow != kInRegisters) wait_async<0>();
+  if (!kWarp && parts > 1) cluster.sync();  // no block leaves while another may still write to it
+  if (!a.partial) return;
+  A* mine = static_cast<A*>(a.partial) + static_cast<long long>(blockIdx.x / parts) * 2 * n;
+  if constexpr (kWarp) {
+    // the block's warps hold the same columns: summed in order through shared memory, one of the two sums
+    // after the other
+    A* add = reinterpret_cast<A*>(dyn);  // [warp][word][element][lane]
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+#pragma unroll
+        for (int j = 0; j < kD; ++j) {
+          const D v = which ? sum_g[i][j] : sum_gx[i][j];
+          add[((local * kN + i) * kV + 2 * j) * 32 + t] = v.lo();
+          add[((local * kN + i) * kV + 2 * j + 1) * 32 + t] = v.hi();
+        }
+      __syncthreads();
+      for (int e = threadIdx.x; e < kN * kV * 32; e += blockDim.x) {
+        A v = add[e];
+        for (int b = 1; b < per_block; ++b) v += add[b * kN * kV * 32 + e];
+        const int lane = e & 31, j = (e >> 5) % kV, i = (e >> 5) / kV, c = (lane + 32 * i) * kV + j;
+        if (c < n) mine[which * n + c] = v;
+      }
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < kN; ++i)
 #pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const A g = Elem<T>::widen(cg[i].v[j]);  // zero behind the row
-        const A xhat = (Elem<T>::widen(cx[i].v[j]) - m) * s;
-        const A u = g * Elem<T>::widen(w[i].v[j]);
-        if ((t + i * width) * kV + j < n) {
-          su += u;
-          sux += u * xhat;
-          sum_g[i][j] += g;
-          sum_gx[i][j] += g * xhat;
-        }
+      for (int j = 0; j < kD; ++j) {
+        const int c = (t + i * width) * kV + 2 * j;
+        if (c < n) { mine[c] = sum_gx[i][j].lo(); mine[n + c] = sum_g[i][j].lo(); }
+        if (c + 1 < n) { mine[c + 1] = sum_gx[i][j].hi(); mine[n + c + 1] = sum_g[i][j].hi(); }
       }
-    block_sum2(su, sux, sm, warps);
-    const A level = su * inv_n, along = sux * inv_n;
-    T* out = grad_in + r * ldi;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int c = (t + i * width) * kV;
-      if (c >= n) break;
-      Pack<T, kV> o;
-#pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const A xhat = (Elem<T>::widen(cx[i].v[j]) - m) * s;
-        const A u = Elem<T>::widen(cg[i].v[j]) * Elem<T>::widen(w[i].v[j]);
-        o.v[j] = Elem<T>::narrow(s * (u - level - xhat * along));
-      }
-      store_pack<T, kV>(out, n, c, o);
-    }
   }
-  if (!partial) return;
-  A* mine = partial + group * 2 * n;
-#pragma unroll
-  for (int i = 0; i < kN; ++i)
-#pragma unroll
-    for (int j = 0; j < kV; ++j) {
-      const int c = (t + i * width) * kV + j;
-      if (c < n) {
-        mine[c] = sum_gx[i][j];
-        mine[n + c] = sum_g[i][j];
-      }
-    }
 }
 
 // rows longer than a block's registers hold, first half: the two sums of every row
@@ -248,7 +394,8 @@ __global__ void __launch_bounds__(512) layernorm_row_sums_kernel(
     const typename Elem<T>::Acc* __restrict__ inv_std, const T* __restrict__ gamma,
     typename Elem<T>::Acc* __restrict__ row_sums, long long rows, int n, long long ldg, long long ldx) {
   using A = typename Elem<T>::Acc;
-  __shared__ A sm[64];
+  __shared__ A sm[2][64];
+  int turn = 0;
   const A inv_n = A(1) / A(n);
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const A m = mean[r], s = inv_std[r];
@@ -258,7 +405,8 @@ __global__ void __launch_bounds__(512) layernorm_row_sums_kernel(
       su += u;
       sux += u * ((Elem<T>::widen(x[r * ldx + c]) - m) * s);
     }
-    block_sum2(su, sux, sm, 16);
+    block_sum2(su, sux, sm[turn], 16);
+    turn ^= 1;
     if (threadIdx.x == 0) {
       row_sums[2 * r] = su * inv_n;
       row_sums[2 * r + 1] = sux * inv_n;
@@ -292,153 +440,167 @@ __global__ void __launch_bounds__(256) layernorm_columns_kernel(
 }
 
 // grad_gamma and grad_beta: the groups' shares added in a fixed order, 32 columns of the 2 n per block,
-// eight threads per column
+// 32 threads per column
 template <typename A>
-__global__ void __launch_bounds__(256) layernorm_join_kernel(const A* __restrict__ partial, int groups, int n,
-                                                             A* __restrict__ grad_gamma, A* __restrict__ grad_beta) {
-  __shared__ A sm[8][32];
+__global__ void __launch_bounds__(1024) layernorm_join_kernel(const A* __restrict__ partial, int groups, int n,
+                                                              A* __restrict__ grad_gamma, A* __restrict__ grad_beta) {
+  __shared__ A sm[32][33];
   const int col = threadIdx.x & 31, lane = threadIdx.x >> 5;
   const long long c = static_cast<long long>(blockIdx.x) * 32 + col, width = 2LL * n;
   A s = 0;
   if (c < width) {
 #pragma unroll 8
-    for (int g = lane; g < groups; g += 8) s += partial[g * width + c];
+    for (int g = lane; g < groups; g += 32) s += partial[g * width + c];
   }
   sm[lane][col] = s;
   __syncthreads();
-  if (lane != 0 || c >= width) return;
-#pragma unroll
-  for (int i = 1; i < 8; ++i) s += sm[i][col];
-  if (c < n) { if (grad_gamma) grad_gamma[c] = s; }
-  else if (grad_beta) grad_beta[c - n] = s;
-}
-
-struct NormArgs {
-  const void *x, *gamma, *beta;
-  void *y, *mean, *inv_std;
-  long long rows, ldx, ldy;
-  int n;
-  double epsilon;
-};
-
-template <typename T, int kV, int kN, bool kWarp>
-void launch_forward_as(const NormArgs& a, unsigned grid, int threads, cudaStream_t st) {
-  using A = typename Elem<T>::Acc;
-  layernorm_kernel<T, kV, kN, kWarp><<<grid, threads, 0, st>>>(
-      static_cast<const T*>(a.x), static_cast<const T*>(a.gamma), static_cast<const T*>(a.beta), static_cast<T*>(a.y),
-      static_cast<A*>(a.mean), static_cast<A*>(a.inv_std), a.rows, a.n, a.ldx, a.ldy, static_cast<A>(a.epsilon));
+  // transposed: a warp now holds the 32 shares of one column
+  s = warp_sum(sm[col][lane]);
+  const long long cc = static_cast<long long>(blockIdx.x) * 32 + lane;
+  if (col != 0 || cc >= width) return;
+  if (cc < n) { if (grad_gamma) grad_gamma[cc] = s; }
+  else if (grad_beta) grad_beta[cc - n] = s;
 }
 
 unsigned grid_of(long long want, long long cap) {
   return static_cast<unsigned>(want < 1 ? 1 : (want < cap ? want : cap));
 }
+int warps_for(int words, int per) { return ((words + per - 1) / per + 31) / 32; }
 
-template <typename T, int kV>
-bool launch_forward_packed(const NormArgs& a, cudaStream_t st) {
-  const long long sms = lib_num_sms();
-  const int packs = (a.n + kV - 1) / kV;
-  if (packs <= 32 * 4) {
-    const unsigned grid = grid_of((a.rows + 7) / 8, sms * 8);
-    if (packs <= 32) launch_forward_as<T, kV, 1, true>(a, grid, 256, st);
-    else if (packs <= 64) launch_forward_as<T, kV, 2, true>(a, grid, 256, st);
-    else launch_forward_as<T, kV, 4, true>(a, grid, 256, st);
-    return true;
-  }
-  // few rows: as many threads as packs, one pack each; many rows: four packs a thread
-  const bool few = a.rows < 2 * sms;
-  const auto threads_for = [&](int per) { return ((packs + per - 1) / per + 31) / 32 * 32; };
-  int per = few ? 1 : 4;
-  while (threads_for(per) > 1024) per *= 2;
-  if (per > 8) return false;
-  const int threads = threads_for(per);
-  const unsigned grid = grid_of(a.rows, sms * (2048 / threads));
-  if (per == 1) launch_forward_as<T, kV, 1, false>(a, grid, threads, st);
-  else if (per == 2) launch_forward_as<T, kV, 2, false>(a, grid, threads, st);
-  else if (per == 4) launch_forward_as<T, kV, 4, false>(a, grid, threads, st);
-  else launch_forward_as<T, kV, 8, false>(a, grid, threads, st);
-  return true;
+// more dynamic shared memory than a kernel gets unasked
+template <typename F> bool allow_shared(F kernel, size_t bytes) {
+  return bytes <= 32 * 1024 ||  // static shared memory counts towards the 48 KB that need no asking
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess;
 }
 
-template <typename T>
-int launch_forward(const NormArgs& a, cudaStream_t st) {
+template <typename T, int kN, bool kWarp, int kMost, int kHow>
+void launch_forward_as(const NormArgs& a, int threads, cudaStream_t st) {
+  const size_t smem = kHow == kInRegisters ? 0 : static_cast<size_t>(kNormAhead<kHow>) * kN * threads * 16;
+  const auto kernel = layernorm_kernel<T, kN, kWarp, kMost, kHow>;
+  if (!allow_shared(kernel, smem)) return;  // the error is read after the launch
+  // blocks that an SM holds, by registers (the launch bounds) and by shared memory
+  long long resident = 768 / threads;
+  const long long fit = 220 * 1024 / static_cast<long long>(smem + 1024);
+  if (resident > fit) resident = fit;
+  const long long want = kWarp ? (a.rows + threads / 32 - 1) / (threads / 32) : a.rows;
+  kernel<<<grid_of(want, lib_num_sms() * (resident < 1 ? 1 : resident)), threads, smem, st>>>(a);
+}
+
+// rows in many: a warp each while four words a thread hold it, then a block
+template <typename T, int kHow> void launch_forward_many(const NormArgs& a, int words, cudaStream_t st) {
+  const int threads = 32 * warps_for(words, 4);
+  if (words <= 32) launch_forward_as<T, 1, true, 128, kHow>(a, 128, st);
+  else if (words <= 64) launch_forward_as<T, 2, true, 128, kHow>(a, 128, st);
+  else if (words <= 128) launch_forward_as<T, 4, true, 128, kHow>(a, 128, st);
+  else if (threads <= 128) launch_forward_as<T, 4, false, 128, kHow>(a, threads, st);
+  else if (threads <= 256) launch_forward_as<T, 4, false, 256, kHow>(a, threads, st);
+  else launch_forward_as<T, 4, false, 1024, kHow>(a, threads, st);
+}
+
+template <typename T> int launch_forward(NormArgs a, cudaStream_t st) {
   using A = typename Elem<T>::Acc;
-  constexpr int kV = kVec16<T>;
-  const bool packed = rows_on_16_bytes<T>(a.x, a.ldx) && rows_on_16_bytes<T>(a.y, a.ldy) &&
-                      rows_on_16_bytes<T>(a.gamma, 0) && rows_on_16_bytes<T>(a.beta, 0);
-  if (packed ? launch_forward_packed<T, kV>(a, st) : launch_forward_packed<T, 1>(a, st)) return 1;
-  layernorm_long_kernel<T><<<grid_of(a.rows, static_cast<long long>(lib_num_sms()) * 2), 1024, 0, st>>>(
-      static_cast<const T*>(a.x), static_cast<const T*>(a.gamma), static_cast<const T*>(a.beta), static_cast<T*>(a.y),
-      static_cast<A*>(a.mean), static_cast<A*>(a.inv_std), a.rows, a.n, a.ldx, a.ldy, static_cast<A>(a.epsilon));
+  a.x_words = rows_on_16_bytes<T>(a.x, a.ldx);
+  a.y_words = rows_on_16_bytes<T>(a.y, a.ldy);
+  a.gamma_words = rows_on_16_bytes<T>(a.gamma, 0);
+  a.beta_words = rows_on_16_bytes<T>(a.beta, 0);
+  const int words = (a.n + kVec16<T> - 1) / kVec16<T>;
+  const long long sms = lib_num_sms();
+  if (words > 4096) {  // over four words for each of 1024 threads
+    layernorm_long_kernel<T><<<grid_of(a.rows, sms * 2), 1024, 0, st>>>(
+        static_cast<const T*>(a.x), static_cast<const T*>(a.gamma), static_cast<const T*>(a.beta), static_cast<T*>(a.y),
+        static_cast<A*>(a.mean), static_cast<A*>(a.inv_std), a.rows, a.n, a.ldx, a.ldy, static_cast<A>(a.epsilon));
+  } else if (a.rows < 4 * sms && words > 32) {
+    // few rows: the latency of one counts, so it gets as many threads as it has words, and nothing comes after it
+    if (words <= 1024) launch_forward_as<T, 1, false, 1024, kInRegisters>(a, 32 * warps_for(words, 1), st);
+    else launch_forward_as<T, 4, false, 1024, kInRegisters>(a, 32 * warps_for(words, 4), st);
+  } else if (a.x_words && a.y_words && a.gamma_words && a.beta_words && a.n % kVec16<T> == 0) {
+    launch_forward_many<T, kByWords>(a, words, st);
+  } else {
+    launch_forward_many<T, sizeof(T) >= 4 ? kByElements : kInRegisters>(a, words, st);
+  }
   return 1;
 }
 
-struct NormGradArgs {
-  const void *grad_out, *x, *mean, *inv_std, *gamma;
-  void *grad_in, *grad_gamma, *grad_beta;
-  long long rows, ldg, ldx, ldi;
-  int n;
-};
+// words a thread holds (0: the row does not fit a cluster's registers), threads, blocks per row, rows at once
+struct GradShape { int per, threads, parts; bool warp; long long groups; };
 
-// threads of a row, packs a thread holds and blocks, for rows that fit into registers; kN = 0: they do not
-struct GradShape { int per, threads; bool warp; unsigned grid; };
-
-template <typename T, int kV> GradShape gradients_shape(const NormGradArgs& a) {
+template <typename T> GradShape gradients_shape(const NormGradArgs& a) {
+  constexpr int kV = kVec16<T>;
   const long long sms = lib_num_sms();
-  const int packs = (a.n + kV - 1) / kV;
-  // registers of a pack: the row and the next row (twice two), the weights, two sums of kV
-  constexpr int kMost = 4;
-  if (packs <= 32 * 2) {
-    const int per = packs <= 32 ? 1 : 2;
-    return {per, 256, true, grid_of((a.rows + 7) / 8, sms * 4)};
+  const int words = (a.n + kV - 1) / kV;
+  constexpr int kN = kGradWords<T>;
+  if (words <= 32 * kN) {
+    const int per = words <= 32 ? 1 : words <= 64 ? 2 : 4;
+    return {per, 128, 1, true, grid_of((a.rows + 3) / 4, sms * (per == kN ? 3 : 4))};
   }
-  const auto threads_for = [&](int per) { return ((packs + per - 1) / per + 31) / 32 * 32; };
-  int per = 2;
-  while (threads_for(per) > 512 && per < kMost) per *= 2;
-  if (threads_for(per) > 512) return {0, 0, false, 0};
-  const int threads = threads_for(per);
-  return {per, threads, false, grid_of(a.rows, sms * (threads <= 128 ? 6 : threads <= 256 ? 3 : 1))};
+  // a block takes 512 words (two or four such blocks share an SM); a wider row takes more blocks, at most
+  // eight
+  int parts = 1;
+  while (parts < 8 && words > 512 * parts) parts *= 2;
+  const int threads = 32 * warps_for((words + parts - 1) / parts, kN);
+  if (threads > 256) return {0, 0, 0, false, 0};
+  return {kN, threads, parts, false, grid_of(a.rows, sms * (threads <= 128 ? 4 : 2) / parts)};
 }
 
-template <typename T, int kV, int kN, bool kWarp>
-void launch_gradients_as(const NormGradArgs& a, const GradShape& q, void* partial, cudaStream_t st) {
-  using A = typename Elem<T>::Acc;
-  layernorm_gradients_kernel<T, kV, kN, kWarp><<<q.grid, q.threads, 0, st>>>(
-      static_cast<const T*>(a.grad_out), static_cast<const T*>(a.x), static_cast<const A*>(a.mean),
-      static_cast<const A*>(a.inv_std), static_cast<const T*>(a.gamma), static_cast<T*>(a.grad_in),
-      static_cast<A*>(partial), a.rows, a.n, a.ldg, a.ldx, a.ldi);
+template <typename T, int kN, bool kWarp, int kHow>
+cudaError_t launch_gradients_as(const NormGradArgs& a, const GradShape& q, cudaStream_t st) {
+  size_t smem = kHow != kInRegisters ? static_cast<size_t>(kRowsAhead<kN, kHow>) * 2 * kN * q.threads * 16 : 0;
+  if (kWarp) {  // the warps' shares are summed there at the end
+    const size_t add = static_cast<size_t>(q.threads) * kN * kVec16<T> * sizeof(typename Elem<T>::Acc);
+    if (add > smem) smem = add;
+  }
+  const auto kernel = layernorm_gradients_kernel<T, kN, kWarp, kHow>;
+  if (!allow_shared(kernel, smem)) return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(q.groups * q.parts));
+  cfg.blockDim = dim3(static_cast<unsigned>(q.threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(q.parts);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <typename T, int kV>
-void launch_gradients_packed(const NormGradArgs& a, const GradShape& q, void* partial, cudaStream_t st) {
-  if (q.warp) {
-    if (q.per == 1) launch_gradients_as<T, kV, 1, true>(a, q, partial, st);
-    else launch_gradients_as<T, kV, 2, true>(a, q, partial, st);
-  } else if (q.per == 2) {
-    launch_gradients_as<T, kV, 2, false>(a, q, partial, st);
-  } else {
-    launch_gradients_as<T, kV, 4, false>(a, q, partial, st);
-  }
+template <typename T, int kHow>
+cudaError_t launch_gradients_shaped(const NormGradArgs& a, const GradShape& q, cudaStream_t st) {
+  if (!q.warp) return launch_gradients_as<T, kGradWords<T>, false, kHow>(a, q, st);
+  if (q.per == 1) return launch_gradients_as<T, 1, true, kHow>(a, q, st);
+  if (q.per == 2) return launch_gradients_as<T, 2, true, kHow>(a, q, st);
+  return launch_gradients_as<T, kGradWords<T>, true, kHow>(a, q, st);
+}
+template <typename T> cudaError_t launch_gradients_any(const NormGradArgs& a, const GradShape& q, cudaStream_t st) {
+  if (a.g_words && a.x_words && a.i_words && a.n % kVec16<T> == 0) return launch_gradients_shaped<T, kByWords>(a, q, st);
+  if constexpr (sizeof(T) >= 4) return launch_gradients_shaped<T, kByElements>(a, q, st);
+  else return launch_gradients_shaped<T, kInRegisters>(a, q, st);
 }
 
 template <typename T>
-int launch_gradients(const NormGradArgs& a, OpScratch& scratch, cudaStream_t st) {
+int launch_gradients(NormGradArgs a, OpScratch& scratch, cudaStream_t st) {
   using A = typename Elem<T>::Acc;
-  constexpr int kV = kVec16<T>;
-  const bool packed = rows_on_16_bytes<T>(a.grad_out, a.ldg) && rows_on_16_bytes<T>(a.x, a.ldx) &&
-                      rows_on_16_bytes<T>(a.grad_in, a.ldi) && rows_on_16_bytes<T>(a.gamma, 0);
-  const GradShape q = packed ? gradients_shape<T, kV>(a) : gradients_shape<T, 1>(a);
+  a.g_words = rows_on_16_bytes<T>(a.grad_out, a.ldg);
+  a.x_words = rows_on_16_bytes<T>(a.x, a.ldx);
+  a.i_words = rows_on_16_bytes<T>(a.grad_in, a.ldi);
+  a.gamma_words = rows_on_16_bytes<T>(a.gamma, 0);
+  const GradShape q = gradients_shape<T>(a);
   const bool weights = a.grad_gamma || a.grad_beta;
   const size_t row_of_sums = 2 * static_cast<size_t>(a.n) * sizeof(A);
   int groups = 0, launches = 1;
-  A* partial = nullptr;
   if (q.per) {
-    groups = static_cast<int>(q.grid) * (q.warp ? q.threads / 32 : 1);
+    groups = static_cast<int>(q.groups);
     if (weights) {
-      partial = reinterpret_cast<A*>(scratch.reserve(groups * row_of_sums, st));
-      if (!partial) return -1;
+      a.partial = scratch.reserve(groups * row_of_sums, st);
+      if (!a.partial) return -1;
     }
-    if (packed) launch_gradients_packed<T, kV>(a, q, partial, st);
-    else launch_gradients_packed<T, 1>(a, q, partial, st);
+    const cudaError_t e = launch_gradients_any<T>(a, q, st);
+    if (e != cudaSuccess) {
+      fprintf(stderr, "[eshkol-b200] layer norm launch failed: %s\n", cudaGetErrorString(e));
+      cudaGetLastError();
+      return -1;
+    }
   } else {
     const long long sms = lib_num_sms();
     const unsigned col_blocks = static_cast<unsigned>((a.n + 255) / 256);
@@ -447,19 +609,19 @@ int launch_gradients(const NormGradArgs& a, OpScratch& scratch, cudaStream_t st)
     uint8_t* base = scratch.reserve(head + (weights ? groups * row_of_sums : 0), st);
     if (!base) return -1;
     A* sums = reinterpret_cast<A*>(base);
-    if (weights) partial = reinterpret_cast<A*>(base + head);
+    if (weights) a.partial = base + head;
     layernorm_row_sums_kernel<T><<<grid_of(a.rows, sms * 4), 512, 0, st>>>(
         static_cast<const T*>(a.grad_out), static_cast<const T*>(a.x), static_cast<const A*>(a.mean),
         static_cast<const A*>(a.inv_std), static_cast<const T*>(a.gamma), sums, a.rows, a.n, a.ldg, a.ldx);
     layernorm_columns_kernel<T><<<dim3(col_blocks, static_cast<unsigned>(groups)), 256, 0, st>>>(
         static_cast<const T*>(a.grad_out), static_cast<const T*>(a.x), static_cast<const A*>(a.mean),
-        static_cast<const A*>(a.inv_std), static_cast<const T*>(a.gamma), sums, static_cast<T*>(a.grad_in), partial, a.rows,
-        a.n, a.ldg, a.ldx, a.ldi);
+        static_cast<const A*>(a.inv_std), static_cast<const T*>(a.gamma), sums, static_cast<T*>(a.grad_in),
+        static_cast<A*>(a.partial), a.rows, a.n, a.ldg, a.ldx, a.ldi);
     launches = 2;
   }
   if (weights) {
-    layernorm_join_kernel<A><<<static_cast<unsigned>((2LL * a.n + 31) / 32), 256, 0, st>>>(
-        partial, groups, a.n, static_cast<A*>(a.grad_gamma), static_cast<A*>(a.grad_beta));
+    layernorm_join_kernel<A><<<static_cast<unsigned>((2LL * a.n + 31) / 32), 1024, 0, st>>>(
+        static_cast<const A*>(a.partial), groups, a.n, static_cast<A*>(a.grad_gamma), static_cast<A*>(a.grad_beta));
     ++launches;
   }
   return launches;
@@ -535,7 +697,7 @@ int eshkol_b200_layernorm_gradients_device(const void* grad_out, const void* x, 
   a.ldi = static_cast<long long>(ld_grad_in ? ld_grad_in : features);
   if (!grad_out || !x || !mean || !inv_std || !grad_in || (grad_in == grad_out && a.ldi != a.ldg) || grad_in == x) return -1;
   a.grad_out = grad_out; a.x = x; a.mean = mean; a.inv_std = inv_std; a.gamma = gamma;
-  a.grad_in = grad_in; a.grad_gamma = grad_gamma; a.grad_beta = grad_beta;
+  a.grad_in = grad_in; a.grad_gamma = grad_gamma; a.grad_beta = grad_beta; a.partial = nullptr;
   a.rows = static_cast<long long>(samples); a.n = static_cast<int>(features);
   OpScratch scratch;
   int launches;
