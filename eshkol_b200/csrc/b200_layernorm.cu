@@ -45,16 +45,15 @@ struct NormArgs {
 // rows are on their way in shared memory: every thread copies the words that it will read itself.
 template <int kHow> constexpr int kNormAhead = kHow == kInRegisters ? 1 : 4;
 
-template <typename T, int kN, bool kWarp, int kMost, int kHow>
-__global__ void __launch_bounds__(kMost, kMost == 128 ? 6 : kMost == 256 ? 3 : 1) layernorm_kernel(const NormArgs a) {  // x and y may be the same
+template <typename T, int kN, bool kWarp, int kThreads, int kHow>
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 256 ? 3 : 1) layernorm_kernel(const NormArgs a) {  // x and y may be the same
   using A = typename Elem<T>::Acc;
   using D = Duo<A>;
   constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kNormAhead<kHow>;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ A sm1[32], sm2[64];
-  const int width = kWarp ? 32 : blockDim.x, warps = kWarp ? 1 : blockDim.x >> 5;
-  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
-  const int per_block = kWarp ? blockDim.x >> 5 : 1, group = kWarp ? threadIdx.x >> 5 : 0;
+  constexpr int width = kWarp ? 32 : kThreads, warps = kWarp ? 1 : kThreads / 32, per_block = kWarp ? kThreads / 32 : 1;
+  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, group = kWarp ? threadIdx.x >> 5 : 0;
   const int n = a.n;
   const T *gamma = static_cast<const T*>(a.gamma), *beta = static_cast<const T*>(a.beta);
   const A inv_n = A(1) / A(n), epsilon = static_cast<A>(a.epsilon);
@@ -72,7 +71,7 @@ __global__ void __launch_bounds__(kMost, kMost == 128 ? 6 : kMost == 256 ? 3 : 1
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
           const int c = (t + i * width) * kV;
-          if (c < n) copy_word<T, kHow>(ring + (stage * kN + i) * blockDim.x, in, c, n);
+          if (c < n) copy_word<T, kHow>(ring + (stage * kN + i) * kThreads, in, c, n);
         }
       }
       commit_async();
@@ -89,7 +88,7 @@ __global__ void __launch_bounds__(kMost, kMost == 128 ? 6 : kMost == 256 ? 3 : 1
       wait_async<kAhead - 1>();
 #pragma unroll
       for (int i = 0; i < kN; ++i)
-        widen_word(take_word<T, kHow>(ring + (stage * kN + i) * blockDim.x, (t + i * width) * kV, n, zero), d[i]);
+        widen_word(take_word<T, kHow>(ring + (stage * kN + i) * kThreads, (t + i * width) * kV, n, zero), d[i]);
       fetch(stage);
       stage = stage + 1 == kAhead ? 0 : stage + 1;
     } else {
@@ -213,8 +212,8 @@ struct NormGradArgs {
 template <typename T> constexpr int kGradWords = sizeof(T) == 2 ? 2 : 4;
 template <int kN, int kHow> constexpr int kRowsAhead = kHow == kInRegisters ? 1 : 4;
 
-template <typename T, int kN, bool kWarp, int kHow>
-__global__ void __launch_bounds__(kWarp ? 128 : 256, kWarp ? 3 : 2) layernorm_gradients_kernel(const NormGradArgs a) {
+template <typename T, int kN, bool kWarp, int kThreads, int kHow>
+__global__ void __launch_bounds__(kThreads, kWarp ? 3 : 512 / kThreads) layernorm_gradients_kernel(const NormGradArgs a) {
   using A = typename Elem<T>::Acc;
   using D = Duo<A>;
   constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kRowsAhead<kN, kHow>;
@@ -224,9 +223,9 @@ __global__ void __launch_bounds__(kWarp ? 128 : 256, kWarp ? 3 : 2) layernorm_gr
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = kWarp ? 1 : static_cast<int>(cluster.num_blocks());
   const int part = kWarp ? 0 : static_cast<int>(cluster.block_rank());
-  const int width = kWarp ? 32 : blockDim.x, warps = kWarp ? 1 : blockDim.x >> 5;
+  constexpr int width = kWarp ? 32 : kThreads, warps = kWarp ? 1 : kThreads / 32, per_block = kWarp ? kThreads / 32 : 1;
   const int t = (kWarp ? threadIdx.x & 31 : threadIdx.x) + part * kN * width;  // word of the first pass
-  const int per_block = kWarp ? blockDim.x >> 5 : 1, local = kWarp ? threadIdx.x >> 5 : 0;
+  const int local = kWarp ? threadIdx.x >> 5 : 0;
   const long long group = static_cast<long long>(blockIdx.x / parts) * per_block + local;
   const long long groups = static_cast<long long>(gridDim.x / parts) * per_block;
   const int n = a.n;
@@ -248,7 +247,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : 256, kWarp ? 3 : 2) layernorm_gr
   }
   Word<T>* ring = reinterpret_cast<Word<T>*>(dyn);  // [stage][x or grad_out][word of the pass][thread]
   const auto place = [&](int stage, int which, int i) {
-    return ring + ((stage * 2 + which) * kN + i) * blockDim.x + threadIdx.x;
+    return ring + ((stage * 2 + which) * kN + i) * kThreads + threadIdx.x;
   };
   Word<T> px[kN], pg[kN];
   A next_m[kAhead], next_s[kAhead];
@@ -368,7 +367,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : 256, kWarp ? 3 : 2) layernorm_gr
           add[((local * kN + i) * kV + 2 * j + 1) * 32 + t] = v.hi();
         }
       __syncthreads();
-      for (int e = threadIdx.x; e < kN * kV * 32; e += blockDim.x) {
+      for (int e = threadIdx.x; e < kN * kV * 32; e += kThreads) {
         A v = add[e];
         for (int b = 1; b < per_block; ++b) v += add[b * kN * kV * 32 + e];
         const int lane = e & 31, j = (e >> 5) % kV, i = (e >> 5) / kV, c = (lane + 32 * i) * kV + j;
@@ -465,7 +464,6 @@ __global__ void __launch_bounds__(1024) layernorm_join_kernel(const A* __restric
 unsigned grid_of(long long want, long long cap) {
   return static_cast<unsigned>(want < 1 ? 1 : (want < cap ? want : cap));
 }
-int warps_for(int words, int per) { return ((words + per - 1) / per + 31) / 32; }
 
 // more dynamic shared memory than a kernel gets unasked
 template <typename F> bool allow_shared(F kernel, size_t bytes) {
@@ -473,28 +471,27 @@ template <typename F> bool allow_shared(F kernel, size_t bytes) {
          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess;
 }
 
-template <typename T, int kN, bool kWarp, int kMost, int kHow>
-void launch_forward_as(const NormArgs& a, int threads, cudaStream_t st) {
-  const size_t smem = kHow == kInRegisters ? 0 : static_cast<size_t>(kNormAhead<kHow>) * kN * threads * 16;
-  const auto kernel = layernorm_kernel<T, kN, kWarp, kMost, kHow>;
+template <typename T, int kN, bool kWarp, int kThreads, int kHow>
+void launch_forward_as(const NormArgs& a, cudaStream_t st) {
+  constexpr size_t smem = kHow == kInRegisters ? 0 : static_cast<size_t>(kNormAhead<kHow>) * kN * kThreads * 16;
+  const auto kernel = layernorm_kernel<T, kN, kWarp, kThreads, kHow>;
   if (!allow_shared(kernel, smem)) return;  // the error is read after the launch
   // blocks that an SM holds, by registers (the launch bounds) and by shared memory
-  long long resident = 768 / threads;
-  const long long fit = 220 * 1024 / static_cast<long long>(smem + 1024);
-  if (resident > fit) resident = fit;
-  const long long want = kWarp ? (a.rows + threads / 32 - 1) / (threads / 32) : a.rows;
-  kernel<<<grid_of(want, lib_num_sms() * (resident < 1 ? 1 : resident)), threads, smem, st>>>(a);
+  constexpr long long by_registers = kThreads <= 256 ? 768 / kThreads : 1, by_shared = 220 * 1024 / (smem + 1024);
+  const long long want = kWarp ? (a.rows + kThreads / 32 - 1) / (kThreads / 32) : a.rows;
+  kernel<<<grid_of(want, lib_num_sms() * (by_registers < by_shared ? by_registers : by_shared)), kThreads, smem, st>>>(a);
 }
 
 // rows in many: a warp each while four words a thread hold it, then a block
 template <typename T, int kHow> void launch_forward_many(const NormArgs& a, int words, cudaStream_t st) {
-  const int threads = 32 * warps_for(words, 4);
-  if (words <= 32) launch_forward_as<T, 1, true, 128, kHow>(a, 128, st);
-  else if (words <= 64) launch_forward_as<T, 2, true, 128, kHow>(a, 128, st);
-  else if (words <= 128) launch_forward_as<T, 4, true, 128, kHow>(a, 128, st);
-  else if (threads <= 128) launch_forward_as<T, 4, false, 128, kHow>(a, threads, st);
-  else if (threads <= 256) launch_forward_as<T, 4, false, 256, kHow>(a, threads, st);
-  else launch_forward_as<T, 4, false, 1024, kHow>(a, threads, st);
+  if (words <= 32) launch_forward_as<T, 1, true, 128, kHow>(a, st);
+  else if (words <= 64) launch_forward_as<T, 2, true, 128, kHow>(a, st);
+  else if (words <= 128) launch_forward_as<T, 4, true, 128, kHow>(a, st);
+  else if (words <= 256) launch_forward_as<T, 2, false, 128, kHow>(a, st);
+  else if (words <= 512) launch_forward_as<T, 4, false, 128, kHow>(a, st);
+  else if (words <= 1024) launch_forward_as<T, 4, false, 256, kHow>(a, st);
+  else if (words <= 2048) launch_forward_as<T, 4, false, 512, kHow>(a, st);
+  else launch_forward_as<T, 4, false, 1024, kInRegisters>(a, st);
 }
 
 template <typename T> int launch_forward(NormArgs a, cudaStream_t st) {
@@ -511,8 +508,10 @@ template <typename T> int launch_forward(NormArgs a, cudaStream_t st) {
         static_cast<A*>(a.mean), static_cast<A*>(a.inv_std), a.rows, a.n, a.ldx, a.ldy, static_cast<A>(a.epsilon));
   } else if (a.rows < 4 * sms && words > 32) {
     // few rows: the latency of one counts, so it gets as many threads as it has words, and nothing comes after it
-    if (words <= 1024) launch_forward_as<T, 1, false, 1024, kInRegisters>(a, 32 * warps_for(words, 1), st);
-    else launch_forward_as<T, 4, false, 1024, kInRegisters>(a, 32 * warps_for(words, 4), st);
+    if (words <= 128) launch_forward_as<T, 1, false, 128, kInRegisters>(a, st);
+    else if (words <= 512) launch_forward_as<T, 1, false, 512, kInRegisters>(a, st);
+    else if (words <= 1024) launch_forward_as<T, 1, false, 1024, kInRegisters>(a, st);
+    else launch_forward_as<T, 4, false, 1024, kInRegisters>(a, st);
   } else if (a.x_words && a.y_words && a.gamma_words && a.beta_words && a.n % kVec16<T> == 0) {
     launch_forward_many<T, kByWords>(a, words, st);
   } else {
@@ -521,39 +520,35 @@ template <typename T> int launch_forward(NormArgs a, cudaStream_t st) {
   return 1;
 }
 
-// words a thread holds (0: the row does not fit a cluster's registers), threads, blocks per row, rows at once
-struct GradShape { int per, threads, parts; bool warp; long long groups; };
+// How a row is dealt out: a warp per row (threads 0), or `parts` blocks of `threads`; groups: rows at once.
+// parts 0: the row does not fit.
+struct GradShape { int per, threads, parts; long long groups; };
 
 template <typename T> GradShape gradients_shape(const NormGradArgs& a) {
-  constexpr int kV = kVec16<T>;
+  constexpr int kV = kVec16<T>, kN = kGradWords<T>;
   const long long sms = lib_num_sms();
   const int words = (a.n + kV - 1) / kV;
-  constexpr int kN = kGradWords<T>;
-  if (words <= 32 * kN) {
-    const int per = words <= 32 ? 1 : words <= 64 ? 2 : 4;
-    return {per, 128, 1, true, grid_of((a.rows + 3) / 4, sms * (per == kN ? 3 : 4))};
-  }
-  // a block takes 512 words (two or four such blocks share an SM); a wider row takes more blocks, at most
-  // eight
-  int parts = 1;
-  while (parts < 8 && words > 512 * parts) parts *= 2;
-  const int threads = 32 * warps_for((words + parts - 1) / parts, kN);
-  if (threads > 256) return {0, 0, 0, false, 0};
-  return {kN, threads, parts, false, grid_of(a.rows, sms * (threads <= 128 ? 4 : 2) / parts)};
+  if (words <= 32 * kN) return {words <= 32 ? 1 : words <= 64 ? 2 : 4, 0, 1, grid_of((a.rows + 3) / 4, sms * 3)};
+  // a block takes up to 512 words; a wider row takes more blocks, at most eight
+  int threads = 64, parts = 1;
+  while (threads < 512 / kN && words > threads * kN) threads *= 2;
+  while (parts < 8 && words > threads * kN * parts) parts *= 2;
+  if (words > threads * kN * parts) return {0, 0, 0, 0};
+  return {kN, threads, parts, grid_of(a.rows, sms * (512 / threads) / parts)};
 }
 
-template <typename T, int kN, bool kWarp, int kHow>
+template <typename T, int kN, bool kWarp, int kThreads, int kHow>
 cudaError_t launch_gradients_as(const NormGradArgs& a, const GradShape& q, cudaStream_t st) {
-  size_t smem = kHow != kInRegisters ? static_cast<size_t>(kRowsAhead<kN, kHow>) * 2 * kN * q.threads * 16 : 0;
+  size_t smem = kHow != kInRegisters ? static_cast<size_t>(kRowsAhead<kN, kHow>) * 2 * kN * kThreads * 16 : 0;
   if (kWarp) {  // the warps' shares are summed there at the end
-    const size_t add = static_cast<size_t>(q.threads) * kN * kVec16<T> * sizeof(typename Elem<T>::Acc);
+    const size_t add = static_cast<size_t>(kThreads) * kN * kVec16<T> * sizeof(typename Elem<T>::Acc);
     if (add > smem) smem = add;
   }
-  const auto kernel = layernorm_gradients_kernel<T, kN, kWarp, kHow>;
+  const auto kernel = layernorm_gradients_kernel<T, kN, kWarp, kThreads, kHow>;
   if (!allow_shared(kernel, smem)) return cudaGetLastError();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(q.groups * q.parts));
-  cfg.blockDim = dim3(static_cast<unsigned>(q.threads));
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -567,10 +562,15 @@ cudaError_t launch_gradients_as(const NormGradArgs& a, const GradShape& q, cudaS
 
 template <typename T, int kHow>
 cudaError_t launch_gradients_shaped(const NormGradArgs& a, const GradShape& q, cudaStream_t st) {
-  if (!q.warp) return launch_gradients_as<T, kGradWords<T>, false, kHow>(a, q, st);
-  if (q.per == 1) return launch_gradients_as<T, 1, true, kHow>(a, q, st);
-  if (q.per == 2) return launch_gradients_as<T, 2, true, kHow>(a, q, st);
-  return launch_gradients_as<T, kGradWords<T>, true, kHow>(a, q, st);
+  constexpr int kN = kGradWords<T>;
+  if (q.threads == 0) {
+    if (q.per == 1) return launch_gradients_as<T, 1, true, 128, kHow>(a, q, st);
+    if (q.per == 2) return launch_gradients_as<T, 2, true, 128, kHow>(a, q, st);
+    return launch_gradients_as<T, kN, true, 128, kHow>(a, q, st);
+  }
+  if (q.threads == 64) return launch_gradients_as<T, kN, false, 64, kHow>(a, q, st);
+  if (q.threads == 128) return launch_gradients_as<T, kN, false, 128, kHow>(a, q, st);
+  return launch_gradients_as<T, kN, false, 512 / kN, kHow>(a, q, st);
 }
 template <typename T> cudaError_t launch_gradients_any(const NormGradArgs& a, const GradShape& q, cudaStream_t st) {
   if (a.g_words && a.x_words && a.i_words && a.n % kVec16<T> == 0) return launch_gradients_shaped<T, kByWords>(a, q, st);
@@ -589,7 +589,7 @@ int launch_gradients(NormGradArgs a, OpScratch& scratch, cudaStream_t st) {
   const bool weights = a.grad_gamma || a.grad_beta;
   const size_t row_of_sums = 2 * static_cast<size_t>(a.n) * sizeof(A);
   int groups = 0, launches = 1;
-  if (q.per) {
+  if (q.parts) {
     groups = static_cast<int>(q.groups);
     if (weights) {
       a.partial = scratch.reserve(groups * row_of_sums, st);
