@@ -9,10 +9,12 @@
 // rows are few, by a cluster of blocks that join their m, s, t and alternatives through distributed
 // shared memory, so there is no workspace and no second launch.
 //
-// Top alternatives cost the pass nothing but the threads' own maxima: the n-th largest of them bounds
-// the n-th largest logit from below, so every alternative lies in the places of a thread whose maximum
-// reaches the bound, and only those threads' places (about n of them) are read again.  Order: larger
-// logit first, equal logits by index, kept exactly by comparing (logit, index) as one key.
+// Top alternatives cost the pass little more than the threads' own maxima: a warp's j-th largest of them,
+// and the least such value of all warps, bounds the n-th largest logit from below when j times the warps
+// reach n, so every alternative lies in the words of a thread whose maximum reaches the bound, and only
+// those threads' words (a few dozen of them) are read again.  Order: larger logit first, equal logits by
+// index, kept exactly by comparing (logit, index) as one key; a candidate's rank is the number of better
+// candidates.
 //
 // Entries of minus infinity have probability zero and add nothing.  A row of nothing else has lse minus
 // infinity, entropy zero and a zero gradient.  NaN or plus infinity makes the row's outputs NaN.
@@ -61,46 +63,14 @@ template <typename K> struct Entry {
 template <typename K> __device__ __forceinline__ bool better(const Entry<K>& a, const Entry<K>& b) {
   return a.key > b.key || (a.key == b.key && a.rank > b.rank);
 }
-template <typename K> __device__ __forceinline__ Entry<K> best_of(const Entry<K>& a, const Entry<K>& b, bool want_better) {
-  return (better(a, b) == want_better) ? a : b;
-}
-template <typename K> __device__ __forceinline__ Entry<K> shfl_xor(const Entry<K>& a, int o) {
-  Entry<K> r;
-  r.key = __shfl_xor_sync(0xffffffffu, a.key, o);
-  r.rank = __shfl_xor_sync(0xffffffffu, a.rank, o);
-  return r;
-}
-// plain keys go through the same networks
-__device__ __forceinline__ uint32_t best_of(uint32_t a, uint32_t b, bool want) { return ((a > b) == want) ? a : b; }
-__device__ __forceinline__ unsigned long long best_of(unsigned long long a, unsigned long long b, bool want) {
-  return ((a > b) == want) ? a : b;
-}
-__device__ __forceinline__ uint32_t shfl_xor(uint32_t a, int o) { return __shfl_xor_sync(0xffffffffu, a, o); }
-__device__ __forceinline__ unsigned long long shfl_xor(unsigned long long a, int o) {
-  return __shfl_xor_sync(0xffffffffu, a, o);
-}
-
-// the last five steps of a bitonic sort: lanes hold a bitonic sequence, afterwards the largest is in lane 0
-template <typename E> __device__ __forceinline__ E merge_down(E e) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) e = best_of(e, shfl_xor(e, o), (lane & o) == 0);
-  return e;
-}
-// 32 values over the lanes, largest first
-template <typename E> __device__ __forceinline__ E sort_down(E e) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int size = 2; size <= 16; size <<= 1) {
-#pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1)
-      e = best_of(e, shfl_xor(e, o), ((lane & o) == 0) == ((lane & size) == 0));
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+    if (other > k) k = other;
   }
-  return merge_down(e);
-}
-// the 32 best of a sorted list over the lanes and another whose places are given backwards
-template <typename E> __device__ __forceinline__ E merge_lists(E list, E other_backwards) {
-  return merge_down(best_of(list, other_backwards, true));
+  return k;
 }
 
 // ------------------------------------------------------------------ running sums
@@ -110,6 +80,14 @@ __device__ __forceinline__ float exp_of(float v) {  // results below 2^-126 are 
   return r;
 }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
+__device__ __forceinline__ Duo<float> exp_both(Duo<float> d) {
+  const Duo<float> w = d * both(1.4426950408889634f);
+  float x, y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(w.lo()));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(w.hi()));
+  return Duo<float>::of(x, y);
+}
+__device__ __forceinline__ Duo<double> exp_both(Duo<double> d) { return {exp(d.x), exp(d.y)}; }
 __device__ __forceinline__ float log_of(float v) { return logf(v); }
 __device__ __forceinline__ double log_of(double v) { return log(v); }
 // v, or the bound when v is below it; NaN stays
@@ -158,7 +136,7 @@ template <typename A> __device__ __forceinline__ Sums<A> warp_joined(Sums<A> a) 
 
 // ------------------------------------------------------------------ a row on the 16-byte grid
 // Place v of a row holds the elements v*kV - shift + (0 .. kV-1), kV of them in one aligned 16-byte
-// word; the first and last place may reach beyond the row and are read element by element.
+// word.  The first and the last place may reach beyond the row; those between lie whole in it.
 template <typename T> struct RowGrid {
   static constexpr int kV = kVec16<T>;
   const T* row;
@@ -168,12 +146,12 @@ template <typename T> struct RowGrid {
     places = (len + shift + kV - 1) / kV;
   }
   __device__ __forceinline__ int first(int place) const { return place * kV - shift; }
-  // whole in the row
   __device__ __forceinline__ bool inside(int place) const { return first(place) >= 0 && first(place) + kV <= n; }
-  __device__ __forceinline__ Pack<T, kV> load(int place, T otherwise) const {
+  __device__ __forceinline__ Word<T> whole(int place) const { return *reinterpret_cast<const Word<T>*>(row + first(place)); }
+  __device__ __forceinline__ Word<T> load(int place, T otherwise) const {
     const int c = first(place);
-    if (c >= 0 && c + kV <= n) return *reinterpret_cast<const Pack<T, kV>*>(row + c);
-    Pack<T, kV> p;
+    if (c >= 0 && c + kV <= n) return whole(place);
+    Word<T> p;
 #pragma unroll
     for (int j = 0; j < kV; ++j) p.v[j] = (c + j >= 0 && c + j < n) ? row[c + j] : otherwise;
     return p;
@@ -186,6 +164,111 @@ template <> __device__ __forceinline__ float minus_infinity<float>() { return -I
 template <> __device__ __forceinline__ __half minus_infinity<__half>() { return __ushort_as_half(0xfc00u); }
 template <> __device__ __forceinline__ __nv_bfloat16 minus_infinity<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80u); }
 
+// ------------------------------------------------------------------ a thread's share of a row
+// What the packed pass cannot take is left to the plain one, element by element: for 16-bit logits the
+// pass replaces minus infinity by the type's lowest value (one packed instruction for two elements), which
+// is right while the reference is far above it, and differences stay finite below 2^119.
+template <typename T> struct Range { static constexpr float kLow = -1e38f, kHigh = 1e36f; };
+template <> struct Range<__half> { static constexpr float kLow = -60000.f, kHigh = 65504.f; };
+
+// the largest of kWords words, NaN passed over
+template <typename T, int kWords> __device__ __forceinline__ typename Elem<T>::Acc largest(const Word<T> (&p)[kWords]) {
+  using A = typename Elem<T>::Acc;
+  if constexpr (std::is_same<T, __half>::value) {
+    __half2 m = *reinterpret_cast<const __half2*>(&p[0]);
+#pragma unroll
+    for (int u = 0; u < kWords; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __hmax2(m, reinterpret_cast<const __half2*>(&p[u])[i]);
+    return fmaxf(__low2float(m), __high2float(m));
+  } else if constexpr (sizeof(T) == 2) {
+    __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&p[0]);
+#pragma unroll
+    for (int u = 0; u < kWords; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __hmax2(m, reinterpret_cast<const __nv_bfloat162*>(&p[u])[i]);
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    A m = minus_infinity<A>();
+#pragma unroll
+    for (int u = 0; u < kWords; ++u)
+#pragma unroll
+      for (int j = 0; j < kVec16<T>; ++j) m = m < p[u].v[j] ? static_cast<A>(p[u].v[j]) : m;
+    return m;
+  }
+}
+// minus infinity replaced by the lowest finite value, NaN kept
+__device__ __forceinline__ Word<__half> without_infinity(Word<__half> p) {
+  __half2* h = reinterpret_cast<__half2*>(&p);
+  const __half2 low = __half2half2(__ushort_as_half(0xfbffu));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
+  return p;
+}
+__device__ __forceinline__ Word<__nv_bfloat16> without_infinity(Word<__nv_bfloat16> p) {
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&p);
+  const __nv_bfloat162 low = __bfloat162bfloat162(__ushort_as_bfloat16(0xff7fu));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
+  return p;
+}
+
+template <typename T> struct Running {
+  using A = typename Elem<T>::Acc;
+  A m, most;        // the reference, the maximum so far
+  Duo<A> s, t;
+  __device__ __forceinline__ void start() {
+    m = lowest<A>();
+    most = minus_infinity<A>();
+    s = t = both(A(0));
+  }
+  __device__ __forceinline__ void move(A to) {
+    const A d = floor_at(m - to, kFar<A>), f = exp_of(d);
+    t = fma2(s, both(d), t) * both(f);
+    s = s * both(f);
+    m = to;
+  }
+  __device__ __forceinline__ void plainly(const Word<T>& p) {
+#pragma unroll
+    for (int j = 0; j < kVec16<T>; ++j) {
+      const A x = Elem<T>::widen(p.v[j]);
+      most = most < x ? x : most;
+      if (x > m) move(x);
+      const A d = floor_at(x - m, kFar<A>), e = exp_of(d);
+      s = s + Duo<A>::of(e, A(0));
+      t = t + Duo<A>::of(e * d, A(0));
+    }
+  }
+  template <int kWords> __device__ __forceinline__ void add(const Word<T> (&p)[kWords]) {
+    const A top = largest<T, kWords>(p);
+    most = most < top ? top : most;
+    if constexpr (sizeof(T) == 2) {
+      if (!(top >= Range<T>::kLow) || most > Range<T>::kHigh) {
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) plainly(p[u]);
+        return;
+      }
+    }
+    // exp(x - m) may grow to exp(4): as exact as below one, and the reference seldom moves
+    if (top > m + kSlack<A>) move(top);
+    const Duo<A> minus = both(-m);
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) {
+      Duo<A> x[kDuos<T>];
+      if constexpr (sizeof(T) == 2) widen_word(without_infinity(p[u]), x);
+      else widen_word(p[u], x);
+#pragma unroll
+      for (int j = 0; j < kDuos<T>; ++j) {
+        Duo<A> d = x[j] + minus;
+        if constexpr (sizeof(T) > 2) d = Duo<A>::of(floor_at(d.lo(), kFar<A>), floor_at(d.hi(), kFar<A>));
+        const Duo<A> e = exp_both(d);
+        s = s + e;
+        t = fma2(e, d, t);
+      }
+    }
+  }
+};
+
 struct LogprobArgs {
   const void* logits;
   const int64_t* tokens;
@@ -195,28 +278,76 @@ struct LogprobArgs {
   int vocab, top;
 };
 
+constexpr int kCandidates = 512;
+
 template <typename T, int kThreads> struct LogprobShared {
   using A = typename Elem<T>::Acc;
   using K = typename KeyOf<T>::type;
   static constexpr int kWarps = kThreads / 32;
   Sums<A> sums[kWarps];
   Sums<A> block;             // this block's, read by the cluster's first block
-  K maxima[kWarps][32];      // the threads' maxima, sorted within their warp
-  K bound;
-  int n_again;
-  uint16_t again[kThreads];  // threads whose places are read again
-  Entry<K> lists[kWarps][32];
-  Entry<K> found[kWarps][32 * kVec16<T>];
-  Entry<K> best[32];         // this block's alternatives, read by the cluster's first block
+  K least[kWarps];
+  int n_again, n_found;
+  uint16_t again[kThreads];  // threads whose words are read again
+  Entry<K> found[kCandidates + kMaxTop];
+  Entry<K> best[kMaxTop];    // this block's alternatives, read by the cluster's first block
+};
+
+// best[0 .. top) from the n candidates in `found`: an entry's place is the number of better ones, counted by
+// a warp.  Between barriers; ends with one.
+template <typename T, int kThreads>
+__device__ __forceinline__ void select_best(LogprobShared<T, kThreads>& sm, int n, int top) {
+  using K = typename KeyOf<T>::type;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = warp; i < n; i += kThreads / 32) {
+    const Entry<K> mine = sm.found[i];
+    int place = 0;
+    for (int j = lane; j < n + lane; j += 32)  // as many turns for every lane
+      place += __popc(__ballot_sync(0xffffffffu, j < n && better(sm.found[j < n ? j : 0], mine)));
+    if (lane == 0 && place < top) sm.best[place] = mine;
+  }
+  if (static_cast<int>(threadIdx.x) >= n && static_cast<int>(threadIdx.x) < top) sm.best[threadIdx.x] = Entry<K>{K(0), 0u};
+  __syncthreads();
+}
+
+// The words of 16 bytes that one thread takes from a row, kGroup at a time and kGroups groups ahead in its
+// places of shared memory (cp.async: no registers, no barrier)
+template <typename T, int kThreads, int kGroup, int kGroups> struct WordStream {
+  const Word<T>* from;   // word 0 of this thread; the next are kThreads words further each
+  Word<T>* places;       // [kGroups][kGroup][kThreads] of the block, this thread's column
+  int count, asked;
+  __device__ __forceinline__ void start(const Word<T>* first, int n, Word<T>* shared) {
+    from = first;
+    count = n;
+    places = shared + threadIdx.x;
+    asked = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) ask(g);
+  }
+  __device__ __forceinline__ void ask(int slot) {
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u)
+      if (asked + u < count) copy_async16(places + (slot * kGroup + u) * kThreads, from + static_cast<long long>(asked + u) * kThreads);
+    asked += kGroup;
+    commit_async();
+  }
+  // the words of the group that was asked for first; its slot is asked again afterwards
+  __device__ __forceinline__ void take(int slot, Word<T> (&p)[kGroup]) {
+    wait_async<kGroups - 1>();
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) p[u] = places[(slot * kGroup + u) * kThreads];
+    ask(slot);
+  }
 };
 
 // One row per cluster; the cluster's blocks take contiguous shares of the row's places.
 template <typename T, int kThreads, bool kTop>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kernel(const LogprobArgs a) {
   using A = typename Elem<T>::Acc;
   using K = typename KeyOf<T>::type;
-  constexpr int kV = kVec16<T>, kWarps = kThreads / 32, kAhead = 4;
+  constexpr int kV = kVec16<T>, kWarps = kThreads / 32, kGroup = 4, kGroups = 3;
   __shared__ LogprobShared<T, kThreads> sm;
+  extern __shared__ __align__(16) unsigned char dyn[];
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   const long long r = blockIdx.x / parts;
@@ -224,159 +355,162 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobA
   const RowGrid<T> grid(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
   const int share = (grid.places + parts - 1) / parts;
   const int lo = min(part * share, grid.places), hi = min(lo + share, grid.places);
+  // the row's ends, where a place is not whole, go to two threads; the whole places to all
+  const bool end0 = lo < hi && !grid.inside(lo), end1 = hi - 1 > lo && !grid.inside(hi - 1);
+  const int wlo = lo + (end0 ? 1 : 0), whi = hi - (end1 ? 1 : 0);
   const T nothing = minus_infinity<T>();
 
-  Sums<A> q{lowest<A>(), A(0), A(0)};
-  A mine = minus_infinity<A>();  // this thread's maximum
-  for (int v0 = lo + tid; v0 < hi; v0 += kAhead * kThreads) {
-    Pack<T, kV> p[kAhead];
+  Running<T> q;
+  q.start();
+  const int count = whi - wlo > tid ? (whi - wlo - tid + kThreads - 1) / kThreads : 0;
+  WordStream<T, kThreads, kGroup, kGroups> words;
+  words.start(reinterpret_cast<const Word<T>*>(grid.row + grid.first(wlo + tid)), count, reinterpret_cast<Word<T>*>(dyn));
+  int slot = 0;
+  for (int k = 0; k < count; k += kGroup) {
+    Word<T> p[kGroup];
+    words.take(slot, p);
+    slot = slot + 1 == kGroups ? 0 : slot + 1;
+    if (k + kGroup > count) {  // the last group: minus infinity adds nothing
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int v = v0 + u * kThreads;
-      if (v < hi) {
-        p[u] = grid.load(v, nothing);
-      } else {
+      for (int u = 0; u < kGroup; ++u)
+        if (k + u >= count) {
 #pragma unroll
-        for (int j = 0; j < kV; ++j) p[u].v[j] = nothing;
-      }
+          for (int j = 0; j < kV; ++j) p[u].v[j] = nothing;
+        }
     }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      A x[kV], most = minus_infinity<A>();
-#pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        x[j] = Elem<T>::widen(p[u].v[j]);
-        most = most < x[j] ? x[j] : most;  // a NaN is passed over
-      }
-      mine = mine < most ? most : mine;
-      // exp(x - m) may grow to exp(4): as exact as below one, and the reference seldom moves
-      if (most > q.m + kSlack<A>) move_reference(q, most);
-#pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const A d = floor_at(x[j] - q.m, kFar<A>);
-        const A e = exp_of(d);
-        q.s += e;
-        q.t += e * d;
-      }
-    }
+    q.template add<kGroup>(p);
   }
-  q = warp_joined(q);
-  if (lane == 0) sm.sums[warp] = q;
-  __syncthreads();
+  wait_async<0>();
+  const A mine = q.most;  // over the whole places
+  if (tid == 0 && end0) q.plainly(grid.load(lo, nothing));
+  if (tid == 32 && end1) q.plainly(grid.load(hi - 1, nothing));
+  {
+    Sums<A> w{q.m, total(q.s), total(q.t)};
+    w = warp_joined(w);
+    if (lane == 0) sm.sums[warp] = w;
+  }
+
+  if (kTop) {
+    // the bound, from the warps whose threads all saw whole places: at least `top` maxima reach it
+    const int full = min((whi - wlo) / 32, kWarps);
+    const bool saw = wlo + tid < whi;
+    const K own = saw ? value_key(mine) : K(0);
+    if (warp < full) {
+      const int rounds = (a.top + full - 1) / full;
+      K left = own, m = K(0);
+      for (int i = 0; i < rounds; ++i) {
+        m = warp_max(left);
+        const unsigned have = __ballot_sync(0xffffffffu, left == m);
+        if (lane == __ffs(have) - 1) left = K(0);
+      }
+      if (lane == 0) sm.least[warp] = m;
+    }
+    if (tid == 0) sm.n_again = sm.n_found = 0;
+    __syncthreads();
+    K bound = full ? sm.least[0] : K(0);
+    for (int w = 1; w < full; ++w) bound = sm.least[w] < bound ? sm.least[w] : bound;
+    if (saw && own >= bound) sm.again[atomicAdd(&sm.n_again, 1)] = static_cast<uint16_t>(tid);
+    __syncthreads();
+    // their words again, spread over all threads; candidates in any order
+    const auto collect = [&](int place, const Entry<K>& worst) {
+      const Word<T> p = grid.load(place, nothing);
+      const int c = grid.first(place);
+#pragma unroll
+      for (int j = 0; j < kV; ++j) {
+        const Entry<K> e{value_key(Elem<T>::widen(p.v[j])), 0xffffffffu - static_cast<uint32_t>(c + j)};
+        // NaN has key 0 and is no alternative; neither is what lies beyond the row
+        if (e.key != K(0) && e.key >= bound && c + j >= 0 && c + j < a.vocab && better(e, worst)) {
+          const int at = atomicAdd(&sm.n_found, 1);
+          if (at < kCandidates) sm.found[at] = e;
+        }
+      }
+    };
+    const Entry<K> none{K(0), 0u};
+    const int turns = (whi - wlo + kThreads - 1) / kThreads, n_again = sm.n_again;
+    for (int i = tid; i < n_again * turns; i += kThreads) {
+      const int place = wlo + sm.again[i / turns] + (i % turns) * kThreads;
+      if (place < whi) collect(place, none);
+    }
+    if (tid == 0 && end0) collect(lo, none);
+    if (tid == 32 && end1) collect(hi - 1, none);
+    __syncthreads();
+    int n = sm.n_found;
+    __syncthreads();  // all have read it before it is used again
+    if (n <= kCandidates) {
+      select_best<T, kThreads>(sm, n, a.top);
+    } else {
+      // more logits reach the bound than there is room for (many equal ones): the places in order, as many
+      // at a time as there is room for, each time against the worst alternative so far
+      constexpr int kPlaces = kCandidates / kV < kThreads ? kCandidates / kV : kThreads;
+      if (tid < kMaxTop) sm.best[tid] = none;
+      if (tid == 0) sm.n_found = 0;
+      __syncthreads();
+      for (int v0 = lo; v0 < hi; v0 += kPlaces) {
+        const Entry<K> worst = sm.best[a.top - 1];
+        if (tid < kPlaces && v0 + tid < hi) collect(v0 + tid, worst);
+        __syncthreads();
+        n = sm.n_found;  // at most kCandidates
+        __syncthreads();
+        if (n) {  // the same for all
+          if (tid < a.top) sm.found[n + tid] = sm.best[tid];
+          __syncthreads();
+          if (tid == 0) sm.n_found = 0;
+          select_best<T, kThreads>(sm, n + a.top, a.top);
+        }
+      }
+    }
+  } else {
+    __syncthreads();
+  }
   if (warp == 0) {
     Sums<A> b = lane < kWarps ? sm.sums[lane] : Sums<A>{lowest<A>(), A(0), A(0)};
     b = warp_joined(b);
     if (lane == 0) sm.block = b;
   }
 
-  if (kTop) {
-    // the bound: the top-th largest of the threads' maxima (nothing, if fewer threads saw any logit)
-    const bool saw = lo + tid < hi;
-    const K own = saw ? value_key(mine) : K(0);
-    sm.maxima[warp][lane] = sort_down(own);
-    if (tid == 0) sm.n_again = 0;
-    __syncthreads();
-    if (warp == 0) {
-      K list = sm.maxima[0][lane];
-#pragma unroll 1
-      for (int w = 1; w < kWarps; ++w) list = merge_lists(list, sm.maxima[w][31 - lane]);
-      const K b = __shfl_sync(0xffffffffu, list, a.top - 1);
-      if (lane == 0) sm.bound = b;
-    }
-    __syncthreads();
-    const K bound = sm.bound;
-    if (saw && own >= bound) sm.again[atomicAdd(&sm.n_again, 1)] = static_cast<uint16_t>(tid);
-    __syncthreads();
-    const int n_again = sm.n_again;  // their order does not matter: entries are ordered by key and index
-    Entry<K> list{K(0), 0u};
-    for (int i = warp; i < n_again; i += kWarps) {
-      const int who = sm.again[i];
-      for (int v0 = lo + who; v0 < hi; v0 += 32 * kThreads) {
-        const int v = v0 + lane * kThreads;
-        const K worst = __shfl_sync(0xffffffffu, list.key, 31);
-        const uint32_t worst_rank = __shfl_sync(0xffffffffu, list.rank, 31);
-        const Entry<K> last{worst, worst_rank};
-        Entry<K> e[kV];
-        unsigned take = 0;
-        if (v < hi) {
-          const Pack<T, kV> p = grid.load(v, nothing);
-          const int c = grid.first(v);
-#pragma unroll
-          for (int j = 0; j < kV; ++j) {
-            e[j].key = value_key(Elem<T>::widen(p.v[j]));
-            e[j].rank = 0xffffffffu - static_cast<uint32_t>(c + j);
-            // NaN has key 0 and is no alternative; neither are places beyond the row
-            if (e[j].key != K(0) && e[j].key >= bound && c + j >= 0 && c + j < a.vocab && better(e[j], last)) take |= 1u << j;
-          }
-        }
-        const int count = __popc(take);
-        int at = count;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += up;
-        }
-        const int total = __shfl_sync(0xffffffffu, at, 31);
-        if (total == 0) continue;
-        at -= count;
-#pragma unroll
-        for (int j = 0; j < kV; ++j)
-          if (take & (1u << j)) sm.found[warp][at++] = e[j];
-        __syncwarp();
-        for (int b = 0; b < total; b += 32) {
-          const Entry<K> c = sort_down(b + lane < total ? sm.found[warp][b + lane] : Entry<K>{K(0), 0u});
-          Entry<K> back;
-          back.key = __shfl_sync(0xffffffffu, c.key, 31 - lane);
-          back.rank = __shfl_sync(0xffffffffu, c.rank, 31 - lane);
-          list = merge_lists(list, back);
-        }
-        __syncwarp();
-      }
-    }
-    sm.lists[warp][lane] = list;
-    __syncthreads();
-    if (warp == 0) {
-      const int used = min(n_again, kWarps);
-#pragma unroll 1
-      for (int w = 1; w < used; ++w) list = merge_lists(list, sm.lists[w][31 - lane]);
-      sm.best[lane] = list;
-    }
-  }
-
   // the cluster's first block joins the others' sums and alternatives
   if (parts > 1) cluster.sync();
   else __syncthreads();
-  if (part == 0 && warp == 0) {
-    Sums<A> all{lowest<A>(), A(0), A(0)};
-    if (lane < parts) all = *cluster.map_shared_rank(&sm.block, lane);
-    all = warp_joined(all);
-    const bool empty = all.s == A(0);
-    const A log_s = log_of(all.s);
-    const A lse = empty ? minus_infinity<A>() : all.m + log_s;
-    if (lane == 0) {
-      if (a.lse) static_cast<A*>(a.lse)[r] = lse;
-      if (a.entropy) static_cast<A*>(a.entropy)[r] = empty ? A(0) : log_s - all.t / all.s;
-      if (a.logprob) {
-        const int64_t token = a.tokens[r];
-        A lp = A(0);  // no token was given
-        if (token >= a.vocab) {
-          lp = A(NAN);
-        } else if (token >= 0) {
-          const A x = Elem<T>::widen(grid.row[token]);
-          // x - lse, by way of the reference: x - m is exact for a likely token where lse is rounded
-          lp = (x == minus_infinity<A>() && lse == lse) ? x : (x - all.m) - log_s;
-        }
-        static_cast<A*>(a.logprob)[r] = lp;
-      }
+  if (part == 0) {
+    if (kTop && parts > 1) {
+      for (int i = tid; i < parts * a.top; i += kThreads)
+        sm.found[i] = *cluster.map_shared_rank(&sm.best[i % a.top], i / a.top);
+      __syncthreads();
+      // empty entries equal one another and would take one place: the index makes them differ, and keeps
+      // them behind every logit
+      for (int i = tid; i < parts * a.top; i += kThreads)
+        if (sm.found[i].key == K(0)) sm.found[i].rank = static_cast<uint32_t>(i);
+      __syncthreads();
+      select_best<T, kThreads>(sm, parts * a.top, a.top);
     }
-    if (kTop) {
-      Entry<K> list = sm.best[lane];
-#pragma unroll 1
-      for (int b = 1; b < parts; ++b) list = merge_lists(list, *cluster.map_shared_rank(&sm.best[31 - lane], b));
-      if (lane < a.top) {
-        const bool none = list.key == K(0);
-        const A x = none ? A(NAN) : static_cast<A>(key_value(list.key));
-        if (a.top_index) a.top_index[r * a.top + lane] = none ? -1 : static_cast<int64_t>(0xffffffffu - list.rank);
+    if (warp == 0) {
+      Sums<A> all{lowest<A>(), A(0), A(0)};
+      if (lane < parts) all = *cluster.map_shared_rank(&sm.block, lane);
+      all = warp_joined(all);
+      const bool empty = all.s == A(0);
+      const A log_s = log_of(all.s);
+      const A lse = empty ? minus_infinity<A>() : all.m + log_s;
+      if (lane == 0) {
+        if (a.lse) static_cast<A*>(a.lse)[r] = lse;
+        if (a.entropy) static_cast<A*>(a.entropy)[r] = empty ? A(0) : log_s - all.t / all.s;
+        if (a.logprob) {
+          const int64_t token = a.tokens[r];
+          A lp = A(0);  // no token was given
+          if (token >= a.vocab) {
+            lp = A(NAN);
+          } else if (token >= 0) {
+            const A x = Elem<T>::widen(grid.row[token]);
+            // x - lse, by way of the reference: x - m is exact for a likely token where lse is rounded
+            lp = (x == minus_infinity<A>() && lse == lse) ? x : (x - all.m) - log_s;
+          }
+          static_cast<A*>(a.logprob)[r] = lp;
+        }
+      }
+      if (kTop && lane < a.top) {
+        const Entry<K> e = sm.best[lane];
+        const bool none = e.key == K(0);
+        const A x = none ? A(NAN) : static_cast<A>(key_value(e.key));
+        if (a.top_index) a.top_index[r * a.top + lane] = none ? -1 : static_cast<int64_t>(0xffffffffu - e.rank);
         if (a.top_logprob)
           static_cast<A*>(a.top_logprob)[r * a.top + lane] =
               (x == minus_infinity<A>() && lse == lse) ? x : (x - all.m) - log_s;
@@ -397,66 +531,86 @@ struct LogprobGradArgs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(256) token_logprobs_gradient_kernel(const LogprobGradArgs a) {
+__global__ void __launch_bounds__(256, 4) token_logprobs_gradient_kernel(const LogprobGradArgs a) {
   using A = typename Elem<T>::Acc;
-  constexpr int kV = kVec16<T>, kAhead = 4;
+  using D = Duo<A>;
+  constexpr int kV = kVec16<T>, kD = kDuos<T>, kGroup = 2, kGroups = 4;
+  extern __shared__ __align__(16) unsigned char dyn[];
   const long long r = blockIdx.x / a.parts;
-  const int part = static_cast<int>(blockIdx.x - r * a.parts);
+  const int part = static_cast<int>(blockIdx.x - r * a.parts), tid = threadIdx.x;
   const T* in = static_cast<const T*>(a.logits) + r * a.ld;
   T* out = static_cast<T*>(a.grad_logits) + r * a.ldg;
   // places on the output's 16-byte grid; the input is read in words too where it lies the same way
   const RowGrid<T> to(out, a.vocab);
-  const RowGrid<T> from(in, a.vocab);
-  const bool same = to.shift == from.shift;
+  const bool same = to.shift == elems_past_boundary(in);
   const int share = (to.places + a.parts - 1) / a.parts;
   const int lo = min(part * share, to.places), hi = min(lo + share, to.places);
+  const bool end0 = lo < hi && !to.inside(lo), end1 = hi - 1 > lo && !to.inside(hi - 1);
+  const int wlo = lo + (end0 ? 1 : 0), whi = hi - (end1 ? 1 : 0);
+  const int count = whi - wlo > tid ? (whi - wlo - tid + 255) / 256 : 0;
   const int64_t token = a.tokens ? a.tokens[r] : -1;
   const A lse = static_cast<const A*>(a.lse)[r];
   A g = (a.grad_logprob && token >= 0) ? static_cast<const A*>(a.grad_logprob)[r] : A(0);
   const A h = a.grad_entropy ? static_cast<const A*>(a.grad_entropy)[r] : A(0);
   const A ent = a.grad_entropy ? static_cast<const A*>(a.entropy)[r] : A(0);
   if (token >= a.vocab) g = A(NAN);  // a token that does not exist: the row says so
-  const A level = g + h * ent;
-  const bool empty = lse == minus_infinity<A>();
-  const T nothing = minus_infinity<T>();
-  for (int v0 = lo + static_cast<int>(threadIdx.x); v0 < hi; v0 += kAhead * 256) {
-    Pack<T, kV> p[kAhead];
+  const bool empty = lse == minus_infinity<A>();  // then every logit is, and every probability zero
+  const D minus_lse = both(empty ? A(0) : -lse), minus_h = both(-h), minus_level = both(-(g + h * ent));
+  // -p (g + h (log p + entropy)) for a pair
+  const auto slope = [&](D x) {
+    D lp = x + minus_lse;
+    lp = D::of(floor_at(lp.lo(), kFar<A>), floor_at(lp.hi(), kFar<A>));
+    return exp_both(lp) * fma2(minus_h, lp, minus_level);
+  };
+  const auto single = [&](T x) { return slope(both(Elem<T>::widen(x))).lo(); };
+  // the token's own element gets g more, with one rounding: by the thread that writes its place, which
+  // keeps the logit in case the result goes over it
+  const int where = (token >= 0 && token < a.vocab) ? static_cast<int>(token) : -1;
+  const int place = where >= 0 ? (where + to.shift) / kV : -1;
+  const bool mine = place >= lo && place < hi &&
+                    tid == (place < wlo ? 0 : place >= whi ? 32 : (place - wlo) & 255);
+  const A peak = mine ? single(in[where]) + g : A(0);
+
+  if (same) {
+    WordStream<T, 256, kGroup, kGroups> words;
+    words.start(reinterpret_cast<const Word<T>*>(in + to.first(wlo + tid)), count, reinterpret_cast<Word<T>*>(dyn));
+    Word<T>* at = reinterpret_cast<Word<T>*>(out + to.first(wlo + tid));
+    int slot = 0;
+    for (int k = 0; k < count; k += kGroup) {
+      Word<T> p[kGroup];
+      words.take(slot, p);
+      slot = slot + 1 == kGroups ? 0 : slot + 1;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int v = v0 + u * 256;
-      if (v >= hi) continue;
-      if (same) {
-        p[u] = from.load(v, nothing);
-      } else {
-        const int c = to.first(v);
+      for (int u = 0; u < kGroup; ++u) {
+        if (k + u >= count) break;
+        D x[kD];
+        widen_word(p[u], x);
 #pragma unroll
-        for (int j = 0; j < kV; ++j) p[u].v[j] = (c + j >= 0 && c + j < a.vocab) ? in[c + j] : nothing;
+        for (int j = 0; j < kD; ++j) x[j] = slope(x[j]);
+        at[static_cast<long long>(k + u) * 256] = to_word<T>(x);
       }
     }
+    wait_async<0>();
+  } else {
+    for (int k = 0; k < count; ++k) {
+      const int c = to.first(wlo + tid + k * 256);
+      Word<T> p;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int v = v0 + u * 256;
-      if (v >= hi) continue;
-      const int c = to.first(v);
-      Pack<T, kV> o;
+      for (int j = 0; j < kV; ++j) p.v[j] = in[c + j];
+      D x[kD];
+      widen_word(p, x);
 #pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const A x = Elem<T>::widen(p[u].v[j]);
-        const A lp = floor_at(x - lse, kFar<A>);
-        const A prob = empty ? A(0) : exp_of(lp);
-        A d = -prob * (h * (empty ? A(0) : lp) + level);
-        if (c + j == token) d += g;
-        o.v[j] = Elem<T>::narrow(d);
-      }
-      if (to.inside(v)) {
-        *reinterpret_cast<Pack<T, kV>*>(out + c) = o;
-      } else {
-#pragma unroll
-        for (int j = 0; j < kV; ++j)
-          if (c + j >= 0 && c + j < a.vocab) out[c + j] = o.v[j];
-      }
+      for (int j = 0; j < kD; ++j) x[j] = slope(x[j]);
+      *reinterpret_cast<Word<T>*>(out + c) = to_word<T>(x);
     }
   }
+  const auto finish_end = [&](int v) {  // a place that is not whole in the row
+    const int c = to.first(v);
+    for (int j = max(0, -c); j < kV && c + j < a.vocab; ++j) out[c + j] = Elem<T>::narrow(single(in[c + j]));
+  };
+  if (tid == 0 && end0) finish_end(lo);
+  if (tid == 32 && end1) finish_end(hi - 1);
+  if (mine) out[where] = Elem<T>::narrow(peak);
 }
 
 int finish(cudaError_t e) {
@@ -474,7 +628,13 @@ cudaError_t launch_parts(const LogprobArgs& a, long long rows, int parts, cudaSt
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kThreads * 12 * 16;  // three groups of four words a thread
   cfg.stream = st;
+  if (kThreads * 12 * 16 > 32 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(token_logprobs_kernel<T, kThreads, kTop>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kThreads * 12 * 16);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = static_cast<unsigned>(parts);
@@ -485,11 +645,14 @@ cudaError_t launch_parts(const LogprobArgs& a, long long rows, int parts, cudaSt
 }
 
 template <typename T> int launch_forward(const LogprobArgs& a, long long rows, cudaStream_t st) {
-  // blocks of a row: as many as give every SM four, while each still has 2048 elements
-  const long long want = (4LL * lib_num_sms() + rows - 1) / rows;
+  // rows that fill the SMs go to a block each; fewer rows to clusters of up to eight larger blocks, as many
+  // as give every SM two of them, while each still has 4096 elements
+  const long long sms = lib_num_sms();
+  if (rows >= 2 * sms || a.vocab < 8192)
+    return finish(a.top ? launch_parts<T, 256, true>(a, rows, 1, st) : launch_parts<T, 256, false>(a, rows, 1, st));
   int parts = 1;
-  while (parts < 8 && parts * 2 <= want && a.vocab / (parts * 2) >= 2048) parts *= 2;
-  return finish(a.top ? launch_parts<T, 256, true>(a, rows, parts, st) : launch_parts<T, 256, false>(a, rows, parts, st));
+  while (parts < 8 && rows * parts * 2 <= 2 * sms && a.vocab / (parts * 2) >= 4096) parts *= 2;
+  return finish(a.top ? launch_parts<T, 512, true>(a, rows, parts, st) : launch_parts<T, 512, false>(a, rows, parts, st));
 }
 
 template <typename T> int launch_gradient(LogprobGradArgs a, long long rows, cudaStream_t st) {
@@ -497,7 +660,7 @@ template <typename T> int launch_gradient(LogprobGradArgs a, long long rows, cud
   int parts = 1;
   while (parts < 64 && parts * 2 <= want && a.vocab / (parts * 2) >= 1024) parts *= 2;
   a.parts = parts;
-  token_logprobs_gradient_kernel<T><<<static_cast<unsigned>(rows * parts), 256, 0, st>>>(a);
+  token_logprobs_gradient_kernel<T><<<static_cast<unsigned>(rows * parts), 256, 256 * 8 * 16, st>>>(a);  // four groups of two words a thread
   return finish(cudaSuccess);
 }
 
