@@ -9,12 +9,11 @@
 // rows are few, by a cluster of blocks that join their m, s, t and alternatives through distributed
 // shared memory, so there is no workspace and no second launch.
 //
-// Top alternatives cost the pass little more than the threads' own maxima: a warp's j-th largest of them,
-// and the least such value of all warps, bounds the n-th largest logit from below when j times the warps
-// reach n, so every alternative lies in the words of a thread whose maximum reaches the bound, and only
-// those threads' words (a few dozen of them) are read again.  Order: larger logit first, equal logits by
-// index, kept exactly by comparing (logit, index) as one key; a candidate's rank is the number of better
-// candidates.
+// Top alternatives cost the pass nothing but the threads' own maxima: the n-th largest of the largest 64 or
+// so of them bounds the n-th largest logit from below, so every alternative lies in the words of a thread
+// whose maximum reaches the bound, and only those threads' words (about n of them) are read again.  Order:
+// larger logit first, equal logits by index, kept exactly by comparing (logit, index) as one key; a
+// candidate's rank is the number of better candidates.
 //
 // Entries of minus infinity have probability zero and add nothing.  A row of nothing else has lse minus
 // infinity, entropy zero and a zero gradient.  NaN or plus infinity makes the row's outputs NaN.
@@ -73,6 +72,38 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
   return k;
 }
 
+// the warp's largest key, taken out of one lane that holds it
+template <typename K> __device__ __forceinline__ K take_largest(K& left) {
+  const K m = warp_max(left);
+  const unsigned have = __ballot_sync(0xffffffffu, left == m);
+  if (static_cast<int>(threadIdx.x & 31) == __ffs(have) - 1) left = K(0);
+  return m;
+}
+template <typename K> __device__ __forceinline__ K exchange(K k, int o, bool larger) {
+  const K other = __shfl_xor_sync(0xffffffffu, k, o);
+  return (k > other) == larger ? k : other;
+}
+// the last steps of a bitonic sort: a bitonic sequence over the lanes becomes one with the largest first
+template <typename K> __device__ __forceinline__ K merge_down(K k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) k = exchange(k, o, (lane & o) == 0);
+  return k;
+}
+template <typename K> __device__ __forceinline__ K sort_down(K k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 16; size <<= 1) {
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) k = exchange(k, o, ((lane & o) == 0) == ((lane & size) == 0));
+  }
+  return merge_down(k);
+}
+// the 32 largest of a sorted list over the lanes and another one, given backwards
+template <typename K> __device__ __forceinline__ K merge_lists(K list, K backwards) {
+  return merge_down(list > backwards ? list : backwards);
+}
+
 // ------------------------------------------------------------------ running sums
 __device__ __forceinline__ float exp_of(float v) {  // results below 2^-126 are zero
   float r;
@@ -80,13 +111,14 @@ __device__ __forceinline__ float exp_of(float v) {  // results below 2^-126 are 
   return r;
 }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
-__device__ __forceinline__ Duo<float> exp_both(Duo<float> d) {
-  const Duo<float> w = d * both(1.4426950408889634f);
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ Duo<float> exp2_both(Duo<float> w) {
   float x, y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(w.lo()));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(w.hi()));
   return Duo<float>::of(x, y);
 }
+__device__ __forceinline__ Duo<float> exp_both(Duo<float> d) { return exp2_both(d * both(kLog2e)); }
 __device__ __forceinline__ Duo<double> exp_both(Duo<double> d) { return {exp(d.x), exp(d.y)}; }
 __device__ __forceinline__ float log_of(float v) { return logf(v); }
 __device__ __forceinline__ double log_of(double v) { return log(v); }
@@ -107,30 +139,20 @@ template <typename A> constexpr A kSlack = A(4);  // how far a value may pass th
 template <typename A> struct Sums {
   A m, s, t;
 };
-template <typename A> __device__ __forceinline__ void move_reference(Sums<A>& a, A m) {
-  const A d = floor_at(a.m - m, kFar<A>);
-  const A f = exp_of(d);
-  a.t = (a.t + d * a.s) * f;
-  a.s *= f;
-  a.m = m;
-}
-template <typename A> __device__ __forceinline__ Sums<A> joined(Sums<A> a, Sums<A> b) {
-  const A m = a.m > b.m ? a.m : b.m;
-  move_reference(a, m);
-  move_reference(b, m);
-  a.s += b.s;
-  a.t += b.t;
-  return a;
-}
+template <typename A> __device__ __forceinline__ Sums<A> nothing_yet() { return {lowest<A>(), A(0), A(0)}; }
+// the sums of the warp's lanes on every lane: the largest reference first, then plain sums
 template <typename A> __device__ __forceinline__ Sums<A> warp_joined(Sums<A> a) {
+  A m = a.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    Sums<A> b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-    a = joined(a, b);
+    const A other = __shfl_xor_sync(0xffffffffu, m, o);
+    m = m < other ? other : m;
   }
+  const A d = floor_at(a.m - m, kFar<A>), f = exp_of(d);
+  a.t = (a.t + d * a.s) * f;
+  a.s *= f;
+  block_sum2(a.s, a.t, static_cast<A*>(nullptr), 1);
+  a.m = m;
   return a;
 }
 
@@ -166,8 +188,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 minus_infinity<__nv_bfloat1
 
 // ------------------------------------------------------------------ a thread's share of a row
 // What the packed pass cannot take is left to the plain one, element by element: for 16-bit logits the
-// pass replaces minus infinity by the type's lowest value (one packed instruction for two elements), which
-// is right while the reference is far above it, and differences stay finite below 2^119.
+// pass replaces minus infinity by a very low value (one packed instruction for two elements), which is
+// right while the reference is far above it and differences stay finite.
 template <typename T> struct Range { static constexpr float kLow = -1e38f, kHigh = 1e36f; };
 template <> struct Range<__half> { static constexpr float kLow = -60000.f, kHigh = 65504.f; };
 
@@ -197,7 +219,7 @@ template <typename T, int kWords> __device__ __forceinline__ typename Elem<T>::A
     return m;
   }
 }
-// minus infinity replaced by the lowest finite value, NaN kept
+// minus infinity replaced by the lowest finite value (bf16: what is below -1.99e38 by that), NaN kept
 __device__ __forceinline__ Word<__half> without_infinity(Word<__half> p) {
   __half2* h = reinterpret_cast<__half2*>(&p);
   const __half2 low = __half2half2(__ushort_as_half(0xfbffu));
@@ -207,7 +229,7 @@ __device__ __forceinline__ Word<__half> without_infinity(Word<__half> p) {
 }
 __device__ __forceinline__ Word<__nv_bfloat16> without_infinity(Word<__nv_bfloat16> p) {
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&p);
-  const __nv_bfloat162 low = __bfloat162bfloat162(__ushort_as_bfloat16(0xff7fu));
+  const __nv_bfloat162 low = __bfloat162bfloat162(__ushort_as_bfloat16(0xff16u));  // -1.99e38: log2 e times it is finite
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
   return p;
@@ -251,19 +273,37 @@ template <typename T> struct Running {
     }
     // exp(x - m) may grow to exp(4): as exact as below one, and the reference seldom moves
     if (top > m + kSlack<A>) move(top);
-    const Duo<A> minus = both(-m);
+    if constexpr (sizeof(T) == 2) {
+      // (x - m) log2 e in one instruction: its rounding, 2^-25 of m log2 e, shifts all of the thread's
+      // exponents alike and comes to about half a step of the f32 result lse; t in units of log 2
+      const Duo<A> minus = both(-m * kLog2e), scale = both(kLog2e);
+      Duo<A> t2 = both(A(0));
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) {
-      Duo<A> x[kDuos<T>];
-      if constexpr (sizeof(T) == 2) widen_word(without_infinity(p[u]), x);
-      else widen_word(p[u], x);
+      for (int u = 0; u < kWords; ++u) {
+        Duo<A> x[kDuos<T>];
+        widen_word(without_infinity(p[u]), x);
 #pragma unroll
-      for (int j = 0; j < kDuos<T>; ++j) {
-        Duo<A> d = x[j] + minus;
-        if constexpr (sizeof(T) > 2) d = Duo<A>::of(floor_at(d.lo(), kFar<A>), floor_at(d.hi(), kFar<A>));
-        const Duo<A> e = exp_both(d);
-        s = s + e;
-        t = fma2(e, d, t);
+        for (int j = 0; j < kDuos<T>; ++j) {
+          const Duo<A> d = fma2(x[j], scale, minus), e = exp2_both(d);
+          s = s + e;
+          t2 = fma2(e, d, t2);
+        }
+      }
+      t = fma2(t2, both(kLn2), t);
+    } else {
+      const Duo<A> minus = both(-m);
+#pragma unroll
+      for (int u = 0; u < kWords; ++u) {
+        Duo<A> x[kDuos<T>];
+        widen_word(p[u], x);
+#pragma unroll
+        for (int j = 0; j < kDuos<T>; ++j) {
+          Duo<A> d = x[j] + minus;
+          d = Duo<A>::of(floor_at(d.lo(), kFar<A>), floor_at(d.hi(), kFar<A>));
+          const Duo<A> e = exp_both(d);
+          s = s + e;
+          t = fma2(e, d, t);
+        }
       }
     }
   }
@@ -278,15 +318,14 @@ struct LogprobArgs {
   int vocab, top;
 };
 
-constexpr int kCandidates = 512;
-
 template <typename T, int kThreads> struct LogprobShared {
   using A = typename Elem<T>::Acc;
   using K = typename KeyOf<T>::type;
   static constexpr int kWarps = kThreads / 32;
+  static constexpr int kCandidates = kThreads == 32 ? 256 : 512;
   Sums<A> sums[kWarps];
   Sums<A> block;             // this block's, read by the cluster's first block
-  K least[kWarps];
+  K largest[64];             // 64 / kWarps of the largest of each warp's maxima
   int n_again, n_found;
   uint16_t again[kThreads];  // threads whose words are read again
   Entry<K> found[kCandidates + kMaxTop];
@@ -346,6 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
   using A = typename Elem<T>::Acc;
   using K = typename KeyOf<T>::type;
   constexpr int kV = kVec16<T>, kWarps = kThreads / 32, kGroup = 4, kGroups = 3;
+  constexpr int kCandidates = LogprobShared<T, kThreads>::kCandidates;
   __shared__ LogprobShared<T, kThreads> sm;
   extern __shared__ __align__(16) unsigned char dyn[];
   cg::cluster_group cluster = cg::this_cluster();
@@ -359,6 +399,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
   const bool end0 = lo < hi && !grid.inside(lo), end1 = hi - 1 > lo && !grid.inside(hi - 1);
   const int wlo = lo + (end0 ? 1 : 0), whi = hi - (end1 ? 1 : 0);
   const T nothing = minus_infinity<T>();
+  // the token's logit is on its way while the row is read
+  int64_t token = -1;
+  T picked = nothing;
+  if (part == 0 && tid == 0 && a.logprob) {
+    token = a.tokens[r];
+    if (token >= 0 && token < a.vocab) picked = grid.row[token];
+  }
 
   Running<T> q;
   q.start();
@@ -382,57 +429,81 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
   }
   wait_async<0>();
   const A mine = q.most;  // over the whole places
+  constexpr int kSecond = kThreads > 32 ? 32 : 0;  // the thread of the other end
   if (tid == 0 && end0) q.plainly(grid.load(lo, nothing));
-  if (tid == 32 && end1) q.plainly(grid.load(hi - 1, nothing));
+  if (tid == kSecond && end1) q.plainly(grid.load(hi - 1, nothing));
   {
-    Sums<A> w{q.m, total(q.s), total(q.t)};
-    w = warp_joined(w);
+    const Sums<A> w = warp_joined(Sums<A>{q.m, total(q.s), total(q.t)});
     if (lane == 0) sm.sums[warp] = w;
   }
 
   if (kTop) {
-    // the bound, from the warps whose threads all saw whole places: at least `top` maxima reach it
-    const int full = min((whi - wlo) / 32, kWarps);
-    const bool saw = wlo + tid < whi;
+    // the bound: at least `top` threads' maxima reach it (zero when there are not so many among the 32)
+    const bool saw = count > 0;
     const K own = saw ? value_key(mine) : K(0);
-    if (warp < full) {
-      const int rounds = (a.top + full - 1) / full;
-      K left = own, m = K(0);
-      for (int i = 0; i < rounds; ++i) {
-        m = warp_max(left);
-        const unsigned have = __ballot_sync(0xffffffffu, left == m);
-        if (lane == __ffs(have) - 1) left = K(0);
+    constexpr int kOfWarp = kWarps > 1 ? 64 / kWarps : 32;
+    const int of_warp = min(a.top, kOfWarp);
+    if (kWarps > 1) {
+      if (a.top <= 8) {
+        K left = own;
+#pragma unroll 1
+        for (int i = 0; i < of_warp; ++i) {
+          const K m = take_largest(left);
+          if (lane == 0) sm.largest[warp * of_warp + i] = m;
+        }
+      } else {
+        const K sorted = sort_down(own);
+        if (lane < of_warp) sm.largest[warp * of_warp + lane] = sorted;
       }
-      if (lane == 0) sm.least[warp] = m;
     }
     if (tid == 0) sm.n_again = sm.n_found = 0;
     __syncthreads();
-    K bound = full ? sm.least[0] : K(0);
-    for (int w = 1; w < full; ++w) bound = sm.least[w] < bound ? sm.least[w] : bound;
+    K bound = K(0);
+    if (kWarps == 1) {
+      bound = __shfl_sync(0xffffffffu, sort_down(own), a.top - 1);
+    } else {
+      const int have = kWarps * of_warp;
+      K first = lane < have ? sm.largest[lane] : K(0);
+      const K second = lane + 32 < have ? sm.largest[lane + 32] : K(0);
+      if (a.top <= 8 && have <= 32) {
+#pragma unroll 1
+        for (int i = 0; i < a.top; ++i) bound = take_largest(first);
+      } else {
+        bound = __shfl_sync(0xffffffffu, merge_lists(sort_down(first), __shfl_sync(0xffffffffu, sort_down(second), 31 - lane)), a.top - 1);
+      }
+    }
     if (saw && own >= bound) sm.again[atomicAdd(&sm.n_again, 1)] = static_cast<uint16_t>(tid);
     __syncthreads();
-    // their words again, spread over all threads; candidates in any order
-    const auto collect = [&](int place, const Entry<K>& worst) {
-      const Word<T> p = grid.load(place, nothing);
-      const int c = grid.first(place);
-#pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const Entry<K> e{value_key(Elem<T>::widen(p.v[j])), 0xffffffffu - static_cast<uint32_t>(c + j)};
-        // NaN has key 0 and is no alternative; neither is what lies beyond the row
-        if (e.key != K(0) && e.key >= bound && c + j >= 0 && c + j < a.vocab && better(e, worst)) {
+    // their words again, a thread's by a warp at a time; candidates in any order.  NaN fails the comparison.
+    const A bound_value = bound == K(0) ? minus_infinity<A>() : static_cast<A>(key_value(bound));
+    const auto consider = [&](A x, int index, const Entry<K>& worst) {
+      if (x >= bound_value) {
+        const Entry<K> e{value_key(x), 0xffffffffu - static_cast<uint32_t>(index)};
+        if (better(e, worst)) {
           const int at = atomicAdd(&sm.n_found, 1);
           if (at < kCandidates) sm.found[at] = e;
         }
       }
     };
+    const auto collect = [&](int place, const Entry<K>& worst) {  // any place
+      const Word<T> p = grid.load(place, nothing);
+      const int c = grid.first(place);
+#pragma unroll
+      for (int j = 0; j < kV; ++j)
+        if (c + j >= 0 && c + j < a.vocab) consider(Elem<T>::widen(p.v[j]), c + j, worst);
+    };
     const Entry<K> none{K(0), 0u};
-    const int turns = (whi - wlo + kThreads - 1) / kThreads, n_again = sm.n_again;
-    for (int i = tid; i < n_again * turns; i += kThreads) {
-      const int place = wlo + sm.again[i / turns] + (i % turns) * kThreads;
-      if (place < whi) collect(place, none);
-    }
+    const int n_again = sm.n_again;
+    for (int i = warp; i < n_again; i += kWarps)
+      for (int place = wlo + sm.again[i] + lane * kThreads; place < whi; place += 32 * kThreads) {
+        const Word<T> p[1] = {grid.whole(place)};
+        if (largest<T, 1>(p) >= bound_value) {
+#pragma unroll
+          for (int j = 0; j < kV; ++j) consider(Elem<T>::widen(p[0].v[j]), grid.first(place) + j, none);
+        }
+      }
     if (tid == 0 && end0) collect(lo, none);
-    if (tid == 32 && end1) collect(hi - 1, none);
+    if (tid == kSecond && end1) collect(hi - 1, none);
     __syncthreads();
     int n = sm.n_found;
     __syncthreads();  // all have read it before it is used again
@@ -462,15 +533,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
   } else {
     __syncthreads();
   }
+  Sums<A> all = nothing_yet<A>();
   if (warp == 0) {
-    Sums<A> b = lane < kWarps ? sm.sums[lane] : Sums<A>{lowest<A>(), A(0), A(0)};
-    b = warp_joined(b);
-    if (lane == 0) sm.block = b;
+    if (kWarps == 1) {
+      all = sm.sums[0];
+    } else {
+      if (lane < kWarps) all = sm.sums[lane];
+      all = warp_joined(all);
+    }
+    if (parts > 1 && lane == 0) sm.block = all;
   }
 
   // the cluster's first block joins the others' sums and alternatives
   if (parts > 1) cluster.sync();
-  else __syncthreads();
   if (part == 0) {
     if (kTop && parts > 1) {
       for (int i = tid; i < parts * a.top; i += kThreads)
@@ -484,9 +559,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
       select_best<T, kThreads>(sm, parts * a.top, a.top);
     }
     if (warp == 0) {
-      Sums<A> all{lowest<A>(), A(0), A(0)};
-      if (lane < parts) all = *cluster.map_shared_rank(&sm.block, lane);
-      all = warp_joined(all);
+      if (parts > 1) {
+        all = nothing_yet<A>();
+        if (lane < parts) all = *cluster.map_shared_rank(&sm.block, lane);
+        all = warp_joined(all);
+      }
       const bool empty = all.s == A(0);
       const A log_s = log_of(all.s);
       const A lse = empty ? minus_infinity<A>() : all.m + log_s;
@@ -494,12 +571,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
         if (a.lse) static_cast<A*>(a.lse)[r] = lse;
         if (a.entropy) static_cast<A*>(a.entropy)[r] = empty ? A(0) : log_s - all.t / all.s;
         if (a.logprob) {
-          const int64_t token = a.tokens[r];
           A lp = A(0);  // no token was given
           if (token >= a.vocab) {
             lp = A(NAN);
           } else if (token >= 0) {
-            const A x = Elem<T>::widen(grid.row[token]);
+            const A x = Elem<T>::widen(picked);
             // x - lse, by way of the reference: x - m is exact for a likely token where lse is rounded
             lp = (x == minus_infinity<A>() && lse == lse) ? x : (x - all.m) - log_s;
           }
@@ -644,15 +720,20 @@ cudaError_t launch_parts(const LogprobArgs& a, long long rows, int parts, cudaSt
   return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, kThreads, kTop>, a);
 }
 
+template <typename T, int kThreads> int launch_with(const LogprobArgs& a, long long rows, int parts, cudaStream_t st) {
+  return finish(a.top ? launch_parts<T, kThreads, true>(a, rows, parts, st) : launch_parts<T, kThreads, false>(a, rows, parts, st));
+}
 template <typename T> int launch_forward(const LogprobArgs& a, long long rows, cudaStream_t st) {
-  // rows that fill the SMs go to a block each; fewer rows to clusters of up to eight larger blocks, as many
-  // as give every SM two of them, while each still has 4096 elements
+  // A row costs a block some microseconds beside its bytes, the more the wider the block: rows that fill
+  // the SMs go to a warp each up to 256 words and to four warps beyond; fewer rows to clusters of up to
+  // eight large blocks, as many as give every SM two of them, while each still has 4096 elements
   const long long sms = lib_num_sms();
-  if (rows >= 2 * sms || a.vocab < 8192)
-    return finish(a.top ? launch_parts<T, 256, true>(a, rows, 1, st) : launch_parts<T, 256, false>(a, rows, 1, st));
+  const int words = a.vocab / kVec16<T>;
+  if (a.top <= 8 && (words <= 64 || (words <= 256 && rows >= 4 * sms))) return launch_with<T, 32>(a, rows, 1, st);
+  if (rows >= 4 * sms || a.vocab < 8192) return launch_with<T, 128>(a, rows, 1, st);
   int parts = 1;
   while (parts < 8 && rows * parts * 2 <= 2 * sms && a.vocab / (parts * 2) >= 4096) parts *= 2;
-  return finish(a.top ? launch_parts<T, 512, true>(a, rows, parts, st) : launch_parts<T, 512, false>(a, rows, parts, st));
+  return launch_with<T, 512>(a, rows, parts, st);
 }
 
 template <typename T> int launch_gradient(LogprobGradArgs a, long long rows, cudaStream_t st) {
