@@ -11,8 +11,8 @@
 // TMEM; a result is rounded to the storage type once.
 //
 // f32 tensors: every value is split into three bf16 numbers (8 + 8 + 8 bits of its significand, exact
-// but for the last rounding, relative 2^-27), and six of the nine products of the parts, the smallest
-// first, make the result; the three left out are below 2^-26 of the terms.
+// but for the last rounding, relative 2^-27), and six of the nine products of the parts make the result;
+// the three left out are below 2^-26 of the terms.
 //
 // Few output tiles and a long reduction: the reduction is split over blocks, their f32 sums go to scratch
 // and a second kernel adds them in order and applies the epilogue.
@@ -30,45 +30,63 @@
 namespace b200 {
 namespace {
 
-constexpr int kLinThreads = 192;
+constexpr int kLinThreads = 320;    // warps 0 and 1 load and issue, eight warps drain
 constexpr int kLinBM = 128;
-constexpr int kLinBK = 64;          // 16-bit elements per k-block: one 128-byte swizzle row
 constexpr int kLinUmmaK = 16;
-constexpr uint32_t kABytes = kLinBM * 128;
-constexpr int kStagePitch = 36;     // f32 per row of a warp's 32 x 32 exchange tile: 16-byte accesses without conflicts
-constexpr uint32_t kExchangeBytes = 4 * 32 * kStagePitch * 4;
+constexpr int kStagePitch = 36;     // f32 per row of a warp's 16 x 32 exchange tile: 16-byte accesses without conflicts
+constexpr int kExchange = 16 * kStagePitch + 128;  // f32 of an epilogue warp: the exchange tile, its columns' bias
+constexpr uint32_t kExchangeBytes = 8 * kExchange * 4;
+constexpr int kMaxWorkers = 160;
 
-template <int BN> struct LinShape {
-  static constexpr uint32_t kBBytes = BN * 128;
-  static constexpr int kStages = 196608 / (kABytes + kBBytes);
-  static constexpr uint32_t kTmem = 2 * BN;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * (kABytes + kBBytes) + kExchangeBytes + 1024;
+// 16-bit operands as they are, f32 as three bf16 planes
+template <typename T> struct Plane { using type = T; static constexpr int kCount = 1; };
+template <> struct Plane<float> { using type = __nv_bfloat16; static constexpr int kCount = 3; };
+
+// The kernel's shape: tiles of 128 x BN, or of 256 x BN by a pair of SMs (cta_group::2), each of which loads
+// 128 rows of A and half of B's columns: per SM a third less to load than a 128 x 256 tile by itself.
+// f32: k-blocks of 32, the three planes of both operands in a stage, so that their six products cost the
+// loads of three; two accumulators, the product of the leading parts in one and the rest, 2^-8 of it, in
+// the other, handed over every kDrain k-blocks and added up in registers: the tensor core truncates its
+// sums, and 16 truncations in a row are as many as the result's accuracy bears (measured: 126 in a row left
+// 2e-6 of the norm, 16 leave 4e-7).
+template <int BN, typename T, bool kPair> struct LinShape {
+  static constexpr int kPlanes = Plane<T>::kCount;
+  static constexpr int kBK = kPlanes == 3 ? 32 : 64;       // elements per k-block: 64- or 128-byte swizzle rows
+  static constexpr int kDrain = kPlanes == 3 ? 8 : 1 << 28;
+  static constexpr int kAccs = kPlanes == 3 ? 2 : 1;
+  static constexpr int kBRows = kPair ? BN / 2 : BN;       // columns of B that this SM loads
+  static constexpr uint32_t kABytes = kLinBM * kBK * 2, kBBytes = kBRows * kBK * 2;
+  static constexpr uint32_t kStageBytes = kPlanes * (kABytes + kBBytes);
+  static constexpr int kStages = 196608 / kStageBytes;
+  static constexpr uint32_t kTmem = 2 * kAccs * BN;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kExchangeBytes + 1024;
 };
 
-constexpr int kMaxSegs = 6;
-
-// One product C[M x N] = sum over segments of A_plane B_plane, and what becomes of it.
-struct LinProduct {
-  int M, N;
-  int kb;                 // k-blocks of a segment
-  int n_seg;
-  int seg_a[kMaxSegs], seg_b[kMaxSegs];
-  int a_mn, b_mn;         // 1: the operand is MN-major
-  int tiles_m, tiles_n, splits, kb_per_split;  // k-blocks over all segments, dealt out to the splits
-  int first_work;         // of this product among the launch's work items
-  float* partial;         // with splits > 1: [splits][M][ldp]
-  long long ldp;
-  // the epilogue (without splits)
+// What becomes of a product's sums
+struct LinEpilogue {
   const void *bias, *residual;
   void *out, *pre;
   long long ldo, ld_res, ld_pre;
-  int act;
+  int M, N, act;
   int words;              // 1: out, pre and residual rows lie on 16-byte boundaries
 };
 
+// One product C[M x N] = A B
+struct LinProduct {
+  LinEpilogue e;
+  int kb;                 // k-blocks
+  int a_mn, b_mn;         // 1: the operand is MN-major
+  int tiles_m, tiles_n, splits, kb_per_split, items;
+  float* partial;         // with splits > 1: [splits][M][ldp]
+  long long ldp;
+};
+
+// The workers (SMs, or pairs) take the first product's items in turn, and then of the second product's
+// items each a share that evens out their work.
 struct LinParams {
   LinProduct p[2];
-  int n_products, total_work;
+  int n_products, workers;
+  int start[kMaxWorkers + 1];  // of the shares
   uint32_t formats;       // operand type bits of the instruction descriptor
   int* status;
   unsigned long long wait_ns;
@@ -82,360 +100,566 @@ struct LinMaps {
 struct LinWork {
   int which, tm, tn, split, kb0, kb1;
 };
-__device__ __forceinline__ LinWork decode(const LinParams& prm, int w) {
-  LinWork it;
-  it.which = (prm.n_products > 1 && w >= prm.p[1].first_work) ? 1 : 0;
-  const LinProduct& q = prm.p[it.which];
-  int t = w - q.first_work;
-  const int tiles = q.tiles_m * q.tiles_n;
-  it.split = t / tiles;
-  t -= it.split * tiles;
-  // groups of 16 tiles along M share the operand B's tiles while they are in L2
-  const int per_group = 16 * q.tiles_n;
-  const int g = t / per_group, r = t - g * per_group;
-  const int gm = min(16, q.tiles_m - g * 16);
-  it.tn = r / gm;
-  it.tm = g * 16 + (r - it.tn * gm);
-  it.kb0 = it.split * q.kb_per_split;
-  it.kb1 = min(it.kb0 + q.kb_per_split, q.kb * q.n_seg);
-  return it;
-}
+// a worker's way through its items, the same for all its warps
+struct LinSchedule {
+  int at0, step, end0, at1, end1;
+  __device__ __forceinline__ LinSchedule(const LinParams& prm, int worker) {
+    at0 = worker;
+    step = prm.workers;
+    end0 = prm.p[0].items;
+    at1 = prm.n_products > 1 ? prm.start[worker] : 0;
+    end1 = prm.n_products > 1 ? prm.start[worker + 1] : 0;
+  }
+  __device__ __forceinline__ bool next(const LinParams& prm, LinWork& it) {
+    int t;
+    if (at0 < end0) {
+      it.which = 0;
+      t = at0;
+      at0 += step;
+    } else if (at1 < end1) {
+      it.which = 1;
+      t = at1++;
+    } else {
+      return false;
+    }
+    const LinProduct& q = prm.p[it.which];
+    const int tiles = q.tiles_m * q.tiles_n;
+    it.split = t / tiles;
+    t -= it.split * tiles;
+    // groups of 8 tiles along M share the operand B's tiles while they are in L2
+    const int per_group = 8 * q.tiles_n;
+    const int g = t / per_group, r = t - g * per_group;
+    const int gm = min(8, q.tiles_m - g * 8);
+    it.tn = r / gm;
+    it.tm = g * 8 + (r - it.tn * gm);
+    it.kb0 = it.split * q.kb_per_split;
+    it.kb1 = min(it.kb0 + q.kb_per_split, q.kb);
+    return true;
+  }
+};
 
-// Shared-memory matrix descriptor, 128-byte swizzle.  K-major: rows of 128 bytes, groups of eight rows
-// 1024 bytes apart.  MN-major: one row holds 64 elements of the M or N axis at one k; eight such rows are
-// 1024 bytes apart (stride offset), the next 64 elements of the axis one box of 64 rows further (leading
-// offset).
-__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int mn) {
-  uint64_t d = umma_desc_k128(saddr);
-  if (mn) d |= static_cast<uint64_t>((64u * 128u) >> 4) << 16;
+// Shared-memory matrix descriptor.  K-major: rows of kBK elements in 128- or 64-byte swizzle rows, groups of
+// eight rows apart by eight times that.  MN-major (128-byte swizzle): one row holds 64 elements of the M or
+// N axis at one k; eight such rows are 1024 bytes apart (stride offset), the next 64 elements of the axis one
+// box of kBK rows further (leading offset).
+template <int kBK> __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int mn) {
+  const bool narrow = kBK == 32 && !mn;
+  uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  if (mn) d |= static_cast<uint64_t>((kBK * 128u) >> 4) << 16;
+  d |= static_cast<uint64_t>((narrow ? 512u : 1024u) >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(narrow ? 4 : 2) << 61;
   return d;
 }
 
+// ------------------------------------------------------------------ pairs of SMs
+__device__ __forceinline__ uint32_t pair_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t leader_address(uint32_t saddr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(saddr));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// the same instruction for one SM and for a pair
+template <bool kPair> struct Tensor;
+template <> struct Tensor<false> {
+  static __device__ __forceinline__ void alloc(uint32_t* slot, uint32_t n) { tmem_alloc(slot, n); tmem_relinquish(); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) { tmem_dealloc(t, n); }
+  static __device__ __forceinline__ void load(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+    tma_load_3d(dst, m, bar, c0, c1, c2);
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    umma_f16(d, a, b, idesc, acc);
+  }
+  static __device__ __forceinline__ void commit(uint64_t* bar) { umma_commit(bar); }
+  static __device__ __forceinline__ void arrive_leader(uint64_t* bar) { mbar_arrive(bar); }
+};
+template <> struct Tensor<true> {
+  static __device__ __forceinline__ void alloc(uint32_t* slot, uint32_t n) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(n) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(n) : "memory");
+  }
+  // into this SM's shared memory, counted on the leader's barrier
+  static __device__ __forceinline__ void load(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];"
+        :
+        : "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(leader_address(smem_u32(bar))), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+  // arrives on the barrier of both SMs (a commit, not a load)
+  static __device__ __forceinline__ void commit(uint64_t* bar) {
+    const uint16_t both_sms = 3;
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"(both_sms)
+        : "memory");
+  }
+  static __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_address(smem_u32(bar))) : "memory");
+  }
+};
+
 // ------------------------------------------------------------------ activations
+// Roundings are written out (no contraction left to the compiler), so that a result does not depend on
+// which other results a call asks for.
 template <bool kExact> __device__ __forceinline__ float logistic(float v) {
-  if (kExact) return 1.f / (1.f + expf(-v));
-  return __fdividef(1.f, 1.f + __expf(-v));  // a few 2^-22: below half a step of the 16-bit results
+  if (kExact) return __fdiv_rn(1.f, __fadd_rn(1.f, expf(-v)));
+  // a few 2^-22: below half a step of the 16-bit results
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(v, -1.4426950408889634f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.f, e)));
+  return r;
 }
 constexpr float kGeluA = 0.7978845608028654f, kGeluB = 0.044715f;
-
+// 2 u(z) = 2 A (z + B z^3)
+__device__ __forceinline__ float gelu_argument(float z) {
+  return __fmul_rn(z, __fmaf_rn(2.f * kGeluA * kGeluB, __fmul_rn(z, z), 2.f * kGeluA));
+}
 // 0 none, 1 ReLU, 2 the tanh form of GELU: z (1 + tanh u) / 2 = z logistic(2 u)
 template <bool kExact> __device__ __forceinline__ float activate(float z, int act) {
   if (act == 1) return z > 0.f ? z : 0.f;
-  if (act == 2) return z * logistic<kExact>(2.f * kGeluA * (z + kGeluB * z * z * z));
+  if (act == 2) return __fmul_rn(z, logistic<kExact>(gelu_argument(z)));
   return z;
 }
-template <bool kExact> __device__ __forceinline__ float activate_slope(float z, int act) {
-  if (act == 1) return z > 0.f ? 1.f : 0.f;
-  if (act == 2) {
-    const float x = z > 20.f ? 20.f : (z < -20.f ? -20.f : z);  // the slope is 1 or 0 beyond; no overflow of x^3
-    const float s = logistic<kExact>(2.f * kGeluA * (x + kGeluB * x * x * x));
-    return s + x * s * (1.f - s) * 2.f * kGeluA * (1.f + 3.f * kGeluB * x * x);
-  }
-  return 1.f;
-}
-
-// kV elements of row `row` from column c: bias, activation, residual, the two results
+// kV elements of a row: bias, activation, residual, the two results
 template <typename T, int kV>
-__device__ __forceinline__ void finish_row(const LinProduct& q, long long row, int c, const float (&acc)[kV],
-                                           const float (&bias)[kV], const Pack<T, kV>& res) {
+__device__ __forceinline__ void finish_elements(const LinEpilogue& e, const float (&acc)[kV], const float (&bias)[kV],
+                                                const Pack<T, kV>& res, Pack<T, kV>& y, Pack<T, kV>& pre) {
   constexpr bool kExact = sizeof(T) == 4;
-  Pack<T, kV> z, y;
 #pragma unroll
   for (int j = 0; j < kV; ++j) {
-    const float v = acc[j] + bias[j];
-    z.v[j] = Elem<T>::narrow(v);
-    float a = activate<kExact>(v, q.act);
-    if (q.residual) a += Elem<T>::widen(res.v[j]);
+    const float z = __fadd_rn(acc[j], bias[j]);
+    float a = activate<kExact>(z, e.act);
+    if (e.residual) a = __fadd_rn(a, Elem<T>::widen(res.v[j]));
+    pre.v[j] = Elem<T>::narrow(z);
     y.v[j] = Elem<T>::narrow(a);
   }
-  T* out = static_cast<T*>(q.out) + row * q.ldo + c;
-  T* pre = q.pre ? static_cast<T*>(q.pre) + row * q.ld_pre + c : nullptr;
-  if (c + kV <= q.N) {
-    *reinterpret_cast<Pack<T, kV>*>(out) = y;
-    if (pre) *reinterpret_cast<Pack<T, kV>*>(pre) = z;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kV; ++j)
-      if (c + j < q.N) {
-        out[j] = y.v[j];
-        if (pre) pre[j] = z.v[j];
-      }
-  }
 }
-template <typename T, int kV>
-__device__ __forceinline__ Pack<T, kV> load_residual(const LinProduct& q, long long row, int c) {
-  Pack<T, kV> p;
-  const T* r = static_cast<const T*>(q.residual) + row * q.ld_res + c;
-  if (c + kV <= q.N) return *reinterpret_cast<const Pack<T, kV>*>(r);
-#pragma unroll
-  for (int j = 0; j < kV; ++j) p.v[j] = (c + j < q.N) ? r[j] : Elem<T>::narrow(0);
-  return p;
-}
-template <typename T, int kV>
-__device__ __forceinline__ void load_bias(const LinProduct& q, int c, float (&b)[kV]) {
-#pragma unroll
-  for (int j = 0; j < kV; ++j)
-    b[j] = (q.bias && c + j < q.N) ? Elem<T>::widen(static_cast<const T*>(q.bias)[c + j]) : 0.f;
+template <typename T> __device__ __forceinline__ float bias_at(const LinEpilogue& e, int c) {
+  return (e.bias && c < e.N) ? Elem<T>::widen(static_cast<const T*>(e.bias)[c]) : 0.f;
 }
 
-// a 32 x 32 block of the accumulator, one row per lane in v, from row0 and column c0 of the result
-template <typename T, int kV>
-__device__ __forceinline__ void finish_block(const LinProduct& q, float* tile, const uint32_t (&v)[32], long long row0, int c0) {
-  const int lane = threadIdx.x & 31;
-  constexpr int kLanesPerRow = 32 / kV, kRows = 32 / kLanesPerRow, kSteps = 32 / kRows;
-  const int c = c0 + (lane % kLanesPerRow) * kV, r = lane / kLanesPerRow;
-  constexpr int kGroup = kSteps < 8 ? kSteps : 8;  // residual words on their way at a time
-  float bias[kV];
-  load_bias<T, kV>(q, c, bias);
-  __syncwarp();
+// A 32 x 32 block of sums, one row per lane in v.  Where rows lie on 16-byte boundaries a lane writes its own
+// row's 64 (f32: 128) bytes: whole sectors, and nothing to exchange.
+template <typename T> constexpr int kRowWords = 32 / kVec16<T>;
+template <typename T>
+__device__ __forceinline__ void load_residual(const LinEpilogue& e, long long row, int c0, Word<T> (&res)[kRowWords<T>]) {
+  if (!e.residual || row >= e.M || c0 + 32 > e.N) return;
+  const Word<T>* from = reinterpret_cast<const Word<T>*>(static_cast<const T*>(e.residual) + row * e.ld_res + c0);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(tile + lane * kStagePitch + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  __syncwarp();
+  for (int w = 0; w < kRowWords<T>; ++w) res[w] = from[w];
+}
+template <typename T>
+__device__ __forceinline__ void finish_words(const LinEpilogue& e, const float* bias, const uint32_t (&v)[32], long long row, int c0,
+                                             const Word<T> (&res)[kRowWords<T>]) {
+  constexpr int kV = kVec16<T>;
+  Word<T>* out = reinterpret_cast<Word<T>*>(static_cast<T*>(e.out) + row * e.ldo + c0);
+  Word<T>* pre = reinterpret_cast<Word<T>*>(static_cast<T*>(e.pre) + row * e.ld_pre + c0);
 #pragma unroll
-  for (int s0 = 0; s0 < kSteps; s0 += kGroup) {
-    Pack<T, kV> res[kGroup];
-    if (q.residual) {
+  for (int w = 0; w < kRowWords<T>; ++w) {
+    float acc[kV], b[kV];
+    Word<T> y, z;
 #pragma unroll
-      for (int s = 0; s < kGroup; ++s) {
-        const long long row = row0 + r + (s0 + s) * kRows;
-        if (row < q.M && c < q.N) res[s] = load_residual<T, kV>(q, row, c);
-      }
+    for (int j = 0; j < kV; j += 4) {  // the same for all lanes
+      const float4 f = *reinterpret_cast<const float4*>(bias + w * kV + j);
+      b[j] = f.x; b[j + 1] = f.y; b[j + 2] = f.z; b[j + 3] = f.w;
     }
 #pragma unroll
-    for (int s = 0; s < kGroup; ++s) {
-      const int in_tile = r + (s0 + s) * kRows;
-      const long long row = row0 + in_tile;
-      float acc[kV];
-      if (kV >= 4) {
-#pragma unroll
-        for (int j = 0; j < kV; j += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(tile + in_tile * kStagePitch + (lane % kLanesPerRow) * kV + j);
-          acc[j] = f.x; acc[j + 1] = f.y; acc[j + 2] = f.z; acc[j + 3] = f.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kV; ++j) acc[j] = tile[in_tile * kStagePitch + (lane % kLanesPerRow) * kV + j];
-      }
-      if (row < q.M && c < q.N) finish_row<T, kV>(q, row, c, acc, bias, res[s]);
+    for (int j = 0; j < kV; ++j) acc[j] = __uint_as_float(v[w * kV + j]);
+    finish_elements<T, kV>(e, acc, b, res[w], y, z);
+    if (row < e.M) {
+      out[w] = y;
+      if (e.pre) pre[w] = z;
     }
   }
 }
-
-// a block of a split reduction's partial sums
-__device__ __forceinline__ void store_partial(const LinProduct& q, float* tile, const uint32_t (&v)[32], int split,
+// Any other block goes through the warp's exchange tile, so that lanes next to each other write elements next
+// to each other.
+template <typename T>
+__device__ __forceinline__ void finish_singly(const LinEpilogue& e, float* tile, const float* bias, const uint32_t (&v)[32],
                                               long long row0, int c0) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
+  const int lane = threadIdx.x & 31, c = c0 + lane;
+  const T* res_at = static_cast<const T*>(e.residual) + row0 * e.ld_res + c;
+  T* out_at = static_cast<T*>(e.out) + row0 * e.ldo + c;
+  T* pre_at = static_cast<T*>(e.pre) + row0 * e.ld_pre + c;
+  const float b[1] = {bias[lane]};
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    __syncwarp();
+    if ((lane >> 4) == half) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(tile + lane * kStagePitch + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  __syncwarp();
-  const int c = c0 + (lane & 7) * 4;
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<uint4*>(tile + (lane & 15) * kStagePitch + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+    __syncwarp();
+    const long long left = e.M - row0 - 16 * half;
+    const int rows = left < 16 ? static_cast<int>(left) : 16;
+    if (c < e.N) {
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 8) {  // eight rows on their way at a time
+        Pack<T, 1> res[8];
 #pragma unroll
-  for (int s = 0; s < 8; ++s) {
-    const int in_tile = (lane >> 3) + 4 * s;
-    const long long row = row0 + in_tile;
-    if (row < q.M && c < q.ldp)  // ldp is N rounded up to 4: whole words
-      *reinterpret_cast<float4*>(q.partial + (static_cast<long long>(split) * q.M + row) * q.ldp + c) =
-          *reinterpret_cast<const float4*>(tile + in_tile * kStagePitch + (lane & 7) * 4);
+        for (int s = 0; s < 8; ++s)
+          if (e.residual && r0 + s < rows) res[s].v[0] = res_at[(16 * half + r0 + s) * e.ld_res];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          if (r0 + s >= rows) break;
+          const float acc[1] = {tile[(r0 + s) * kStagePitch + lane]};
+          Pack<T, 1> y, z;
+          finish_elements<T, 1>(e, acc, b, res[s], y, z);
+          out_at[(16 * half + r0 + s) * e.ldo] = y.v[0];
+          if (e.pre) pre_at[(16 * half + r0 + s) * e.ld_pre] = z.v[0];
+        }
+      }
+    }
   }
 }
 
-template <int BN, typename T>
+// a block of a split reduction's partial sums: whole words, ldp is N rounded up to 4
+__device__ __forceinline__ void store_partial(const LinProduct& q, const uint32_t (&v)[32], int split, long long row, int c0) {
+  if (row >= q.e.M) return;
+  float* to = q.partial + (static_cast<long long>(split) * q.e.M + row) * q.ldp + c0;
+#pragma unroll
+  for (int j = 0; j < 32; j += 4)
+    if (c0 + j < q.ldp) *reinterpret_cast<uint4*>(to + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+}
+
+template <int BN, typename T, bool kPair>
 __global__ void __launch_bounds__(kLinThreads, 1)
 linear_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__ LinParams prm) {
-  using Shape = LinShape<BN>;
-  constexpr int kStages = Shape::kStages;
-  constexpr uint32_t kBBytes = Shape::kBBytes;
+  using Shape = LinShape<BN, T, kPair>;
+  using Tc = Tensor<kPair>;
+  constexpr int kStages = Shape::kStages, kBK = Shape::kBK, kPlanes = Shape::kPlanes, kAccs = Shape::kAccs;
+  constexpr uint32_t kABytes = Shape::kABytes, kBBytes = Shape::kBBytes, kStageBytes = Shape::kStageBytes;
   extern __shared__ uint8_t smem_dyn[];
-  __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full_bar[kStages];   // the pair's leader: all loads of a stage landed
+  __shared__ uint64_t empty_bar[kStages];  // the products that read a stage are done
+  __shared__ uint64_t acc_full[2];         // an accumulator is complete
+  __shared__ uint64_t acc_empty[2];        // the pair's leader: an accumulator was drained
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // the same for the whole warp, and known to be
+  const uint32_t rank = kPair ? pair_rank() : 0u;
+  const int worker = kPair ? blockIdx.x >> 1 : blockIdx.x;
   const uint32_t dyn_addr = smem_u32(smem_dyn);
   const uint32_t tile_base = (dyn_addr + 1023u) & ~1023u;
   uint8_t* tiles = smem_dyn + (tile_base - dyn_addr);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 128); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], kPair ? 512 : 256); }
     abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
   }
-  if (warp == 1) {
-    tmem_alloc(&tmem_slot, Shape::kTmem);
-    tmem_relinquish();
-  }
+  if (warp == 1) Tc::alloc(&tmem_slot, Shape::kTmem);
   tc_fence_before();
   __syncthreads();
+  if (kPair) pair_sync();  // the other SM's barriers exist before anything is signalled on them
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  LinSchedule schedule(prm, worker);
+  LinWork it;
 
+  // The loading and the issuing warp go through their loops as whole warps, and one elected lane issues:
+  // descriptors and addresses then live in uniform registers.  With the loops inside one lane's branch they
+  // had to be moved there for every instruction, and the tensor pipe waited a third of the time.
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, issued = 0, last_parity = 0;
-      bool ok = true;
-      int withhold = prm.withhold && blockIdx.x == 0;
-      for (int w = blockIdx.x; w < prm.total_work && ok; w += gridDim.x) {
-        const LinWork it = decode(prm, w);
-        const LinProduct& q = prm.p[it.which];
-        const CUtensorMap* ma = &maps.a[it.which];
-        const CUtensorMap* mb = &maps.b[it.which];
-        int seg = it.kb0 / q.kb, kb = it.kb0 - seg * q.kb;
-        for (int i = it.kb0; i < it.kb1; ++i) {
-          if (!mbar_wait<false>(&empty_bar[stage], phase ^ 1u, &abort_flag, prm.wait_ns)) {
-            atomicCAS(prm.status, kStatusOk, kStatusProducerTimeout);
-            abort_flag = 1;
-            ok = false;
-            break;
-          }
-          if (withhold) {  // tests only: this stage never arrives and the waits behind it run out
-            withhold = 0;
-            if (++stage == kStages) { stage = 0; phase ^= 1u; }
-            if (++kb == q.kb) { kb = 0; ++seg; }
-            continue;
-          }
-          mbar_arrive_expect_tx(&full_bar[stage], kABytes + kBBytes);
-          uint8_t* sa = tiles + stage * kABytes;
-          uint8_t* sb = tiles + kStages * kABytes + stage * kBBytes;
-          const int k0 = kb * kLinBK, m0 = it.tm * kLinBM, n0 = it.tn * BN, pa = q.seg_a[seg], pb = q.seg_b[seg];
-          if (q.a_mn) {
-#pragma unroll
-            for (int j = 0; j < kLinBM / 64; ++j) tma_load_3d(sa + j * 8192, ma, &full_bar[stage], m0 + 64 * j, k0, pa);
-          } else {
-            tma_load_3d(sa, ma, &full_bar[stage], k0, m0, pa);
-          }
-          if (q.b_mn) {
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_load_3d(sb + j * 8192, mb, &full_bar[stage], n0 + 64 * j, k0, pb);
-          } else {
-            tma_load_3d(sb, mb, &full_bar[stage], k0, n0, pb);
-          }
-          issued |= 1u << stage;
-          last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
-          if (++kb == q.kb) { kb = 0; ++seg; }
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, last_parity = 0;
+    bool ok = true;
+    int withhold = prm.withhold && blockIdx.x == 0;
+    while (ok && schedule.next(prm, it)) {
+      const LinProduct& q = prm.p[it.which];
+      const CUtensorMap* ma = &maps.a[it.which];
+      const CUtensorMap* mb = &maps.b[it.which];
+      const bool a_mn = q.a_mn != 0, b_mn = q.b_mn != 0;
+      const int m0 = (kPair ? 2 * it.tm + static_cast<int>(rank) : it.tm) * kLinBM;
+      const int n0 = it.tn * BN + static_cast<int>(rank) * Shape::kBRows;
+      for (int i = it.kb0; i < it.kb1; ++i) {
+        const bool come = mbar_wait<false>(&empty_bar[stage], phase ^ 1u, &abort_flag, prm.wait_ns);
+        if (!__all_sync(0xffffffffu, come)) {
+          atomicCAS(prm.status, kStatusOk, kStatusProducerTimeout);
+          abort_flag = 1;
+          ok = false;
+          break;
         }
-      }
-      if (!ok || abort_flag) {  // leaving early: the copies in flight land first
-        int none = 0;
-        for (int s = 0; s < kStages; ++s)
-          if (issued & (1u << s)) mbar_wait<true>(&full_bar[s], (last_parity >> s) & 1u, &none, prm.wait_ns);
+        if (withhold) {  // tests only: this stage never arrives and the waits behind it run out
+          withhold = 0;
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          continue;
+        }
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], (kPair ? 2u : 1u) * kStageBytes);
+          uint8_t* sa = tiles + stage * kStageBytes;
+          uint8_t* sb = sa + kPlanes * kABytes;
+          const int k0 = i * kBK;
+#pragma unroll
+          for (int pl = 0; pl < kPlanes; ++pl) {
+            if (a_mn) {
+#pragma unroll
+              for (int j = 0; j < kLinBM / 64; ++j)
+                Tc::load(sa + pl * kABytes + j * (kBK * 128), ma, &full_bar[stage], m0 + 64 * j, k0, pl);
+            } else {
+              Tc::load(sa + pl * kABytes, ma, &full_bar[stage], k0, m0, pl);
+            }
+            if (b_mn) {
+#pragma unroll
+              for (int j = 0; j < Shape::kBRows / 64; ++j)
+                Tc::load(sb + pl * kBBytes + j * (kBK * 128), mb, &full_bar[stage], n0 + 64 * j, k0, pl);
+            } else {
+              Tc::load(sb + pl * kBBytes, mb, &full_bar[stage], k0, n0, pl);
+            }
+          }
+        }
+        __syncwarp();
+        issued |= 1u << stage;
+        last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
     }
+    if ((!ok || abort_flag) && rank == 0) {
+      // leaving early: the copies in flight land first (a pair's all count on the leader's barriers, and
+      // the other SM cannot leave before the leader does)
+      int none = 0;
+      for (int s = 0; s < kStages; ++s)
+        if (issued & (1u << s)) mbar_wait<true>(&full_bar[s], (last_parity >> s) & 1u, &none, prm.wait_ns);
+    }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    // ------------------------------------------------------------ MMA issuer (of a pair: the leader's)
+    if (rank == 0) {
       int stage = 0;
       uint32_t phase = 0, unit = 0;
       bool ok = true;
-      for (int w = blockIdx.x; w < prm.total_work && ok; w += gridDim.x) {
-        const LinWork it = decode(prm, w);
+      while (ok && schedule.next(prm, it)) {
         const LinProduct& q = prm.p[it.which];
-        const uint32_t idesc = umma_idesc_f16(kLinBM, BN) | prm.formats | (static_cast<uint32_t>(q.a_mn) << 15) |
-                               (static_cast<uint32_t>(q.b_mn) << 16);
+        const int a_mn = q.a_mn, b_mn = q.b_mn;
+        const uint32_t idesc = umma_idesc_f16(kPair ? 256 : kLinBM, BN) | prm.formats | (static_cast<uint32_t>(a_mn) << 15) |
+                               (static_cast<uint32_t>(b_mn) << 16);
         // an instruction's 16 steps of k: 32 bytes along a K-major row, 16 rows of an MN-major box
-        const uint32_t step_a = q.a_mn ? (16u * 128u) >> 4 : 2u, step_b = q.b_mn ? (16u * 128u) >> 4 : 2u;
-        const uint32_t buf = unit & 1u, aphase = (unit >> 1) & 1u;
-        if (!mbar_wait<false>(&acc_empty[buf], aphase ^ 1u, &abort_flag, prm.wait_ns)) {
-          atomicCAS(prm.status, kStatusOk, kStatusMmaTimeout);
-          abort_flag = 1;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + buf * BN;
-        for (int i = it.kb0; i < it.kb1; ++i) {
-          if (!mbar_wait<false>(&full_bar[stage], phase, &abort_flag, prm.wait_ns)) {
+        const uint32_t step_a = a_mn ? (16u * 128u) >> 4 : 2u, step_b = b_mn ? (16u * 128u) >> 4 : 2u;
+        const uint64_t desc_a = operand_desc<kBK>(tile_base, a_mn), desc_b = operand_desc<kBK>(tile_base + kPlanes * kABytes, b_mn);
+        for (int i0 = it.kb0; i0 < it.kb1 && ok; i0 += Shape::kDrain) {
+          const int i1 = it.kb1 - i0 > Shape::kDrain ? i0 + Shape::kDrain : it.kb1;
+          const uint32_t buf = unit & 1u, aphase = (unit >> 1) & 1u;
+          bool come = mbar_wait<false>(&acc_empty[buf], aphase ^ 1u, &abort_flag, prm.wait_ns);
+          if (!__all_sync(0xffffffffu, come)) {
             atomicCAS(prm.status, kStatusOk, kStatusMmaTimeout);
             abort_flag = 1;
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t da = operand_desc(tile_base + stage * kABytes, q.a_mn);
-          const uint64_t db = operand_desc(tile_base + kStages * kABytes + stage * kBBytes, q.b_mn);
+          const uint32_t d_tmem = tmem_base + buf * kAccs * BN;
+          for (int i = i0; i < i1; ++i) {
+            come = mbar_wait<false>(&full_bar[stage], phase, &abort_flag, prm.wait_ns);
+            if (!__all_sync(0xffffffffu, come)) {
+              atomicCAS(prm.status, kStatusOk, kStatusMmaTimeout);
+              abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t da = desc_a + stage * (kStageBytes >> 4), db = desc_b + stage * (kStageBytes >> 4);
+            if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kLinBK / kLinUmmaK; ++k)
-            umma_f16(d_tmem, da + step_a * k, db + step_b * k, idesc, (i > it.kb0 || k > 0) ? 1u : 0u);
-          umma_commit(&empty_bar[stage]);
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+              for (int k = 0; k < kBK / kLinUmmaK; ++k) {
+                const uint32_t on = (i > i0 || k > 0) ? 1u : 0u;
+                if constexpr (kPlanes == 1) {
+                  Tc::mma(d_tmem, da + step_a * k, db + step_b * k, idesc, on);
+                } else {
+                  // the parts' products: the five small ones beside the large one
+                  constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+                  for (int s = 0; s < 6; ++s)
+                    Tc::mma(d_tmem + (s < 5 ? BN : 0), da + pa[s] * (kABytes >> 4) + step_a * k,
+                            db + pb[s] * (kBBytes >> 4) + step_b * k, idesc, (s == 0 || s == 5) ? on : 1u);
+                }
+              }
+              Tc::commit(&empty_bar[stage]);
+              if (i + 1 == i1) Tc::commit(&acc_full[buf]);
+            }
+            __syncwarp();
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          }
+          ++unit;
         }
-        if (ok) umma_commit(&acc_full[buf]);
-        ++unit;
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int quarter = warp & 3;
-    float* tile = reinterpret_cast<float*>(tiles + static_cast<size_t>(kStages) * (kABytes + kBBytes)) +
-                  quarter * 32 * kStagePitch;
-    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    // a warp reads the quarter of the accumulator's rows that its number allows; two warps share the columns
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
+    constexpr int kBlocks = BN / 64;  // of 32 columns, for each of them
+    const int lane = threadIdx.x & 31;
+    float* tile = reinterpret_cast<float*>(tiles + static_cast<size_t>(kStages) * kStageBytes) + (warp - 2) * kExchange;
+    float* bias = tile + 16 * kStagePitch;  // of the tile's columns, as f32
+    const uint32_t lane_addr = (static_cast<uint32_t>(quarter * 32) << 16) + part * (BN / 2);
     uint32_t unit = 0;
-    for (int w = blockIdx.x; w < prm.total_work; w += gridDim.x) {
-      const LinWork it = decode(prm, w);
+    bool ok = true;
+    const auto wait_full = [&]() {
+      if (mbar_wait<true>(&acc_full[unit & 1u], (unit >> 1) & 1u, &abort_flag, prm.wait_ns)) {
+        tc_fence_after();
+        return true;
+      }
+      atomicCAS(prm.status, kStatusOk, kStatusEpilogueTimeout);
+      abort_flag = 1;
+      return false;
+    };
+    while (ok && schedule.next(prm, it)) {
       const LinProduct& q = prm.p[it.which];
-      const uint32_t buf = unit & 1u, aphase = (unit >> 1) & 1u;
-      if (!mbar_wait<true>(&acc_full[buf], aphase, &abort_flag, prm.wait_ns)) {
-        atomicCAS(prm.status, kStatusOk, kStatusEpilogueTimeout);
-        abort_flag = 1;
-        break;
+      const LinEpilogue e = q.e;
+      const long long row0 = static_cast<long long>(kPair ? 2 * it.tm + static_cast<int>(rank) : it.tm) * kLinBM + quarter * 32;
+      const long long row = row0 + lane;
+      const int n0 = it.tn * BN + part * (BN / 2);
+      const bool whole = q.splits == 1;
+      // what the tile needs beside its sums is fetched while they are still being made
+      Word<T> res[kRowWords<T>];
+      if (whole) {
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < BN / 2; c += 32) bias[c + lane] = bias_at<T>(e, n0 + c + lane);
+        __syncwarp();
+        if (e.words) load_residual<T>(e, row, n0, res);
       }
-      tc_fence_after();
-      const long long row0 = static_cast<long long>(it.tm) * kLinBM + quarter * 32;
-      const int n0 = it.tn * BN;
-#pragma unroll 1
-      for (int cc = 0; cc < BN / 32; ++cc) {
+      const auto store = [&](const uint32_t (&v)[32], int cc) {
         const int c0 = n0 + cc * 32;
-        if (row0 >= q.M || c0 >= q.N) break;  // the same for the whole warp
-        uint32_t v[32];
-        tmem_ld32(tmem_base + lane_addr + buf * BN + cc * 32, v);
-        tmem_ld_wait();
-        if (q.splits > 1) store_partial(q, tile, v, it.split, row0, c0);
-        else if (q.words) finish_block<T, kVec16<T>>(q, tile, v, row0, c0);
-        else finish_block<T, 1>(q, tile, v, row0, c0);
+        if (!whole) {
+          store_partial(q, v, it.split, row, c0);
+        } else if (e.words && c0 + 32 <= e.N) {
+          Word<T> now[kRowWords<T>];
+#pragma unroll
+          for (int w = 0; w < kRowWords<T>; ++w) now[w] = res[w];
+          if (cc + 1 < kBlocks) load_residual<T>(e, row, c0 + 32, res);  // the next block's
+          finish_words<T>(e, bias + cc * 32, v, row, c0, now);
+        } else {
+          finish_singly<T>(e, tile, bias + cc * 32, v, row0, c0);
+        }
+      };
+      if constexpr (kPlanes == 1) {
+        if (!(ok = wait_full())) break;
+#pragma unroll 1
+        for (int cc = 0; cc < kBlocks; ++cc) {
+          if (row0 >= e.M || n0 + cc * 32 >= e.N) break;  // the same for the whole warp
+          uint32_t v[32];
+          tmem_ld32(tmem_base + lane_addr + (unit & 1u) * BN + cc * 32, v);
+          tmem_ld_wait();
+          store(v, cc);
+        }
+        tc_fence_before();
+        Tc::arrive_leader(&acc_empty[unit & 1u]);
+        ++unit;
+      } else {
+        float acc[kBlocks][32];
+#pragma unroll
+        for (int cc = 0; cc < kBlocks; ++cc)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[cc][j] = 0.f;
+        for (int i0 = it.kb0; i0 < it.kb1; i0 += Shape::kDrain) {
+          if (!(ok = wait_full())) break;
+#pragma unroll
+          for (int cc = 0; cc < kBlocks; ++cc) {
+            uint32_t v[32];
+            tmem_ld32(tmem_base + lane_addr + (unit & 1u) * 2 * BN + BN + cc * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[cc][j] += __uint_as_float(v[j]);
+            tmem_ld32(tmem_base + lane_addr + (unit & 1u) * 2 * BN + cc * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[cc][j] += __uint_as_float(v[j]);
+          }
+          tc_fence_before();
+          Tc::arrive_leader(&acc_empty[unit & 1u]);
+          ++unit;
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int cc = 0; cc < kBlocks; ++cc) {
+          if (row0 < e.M && n0 + cc * 32 < e.N) {
+            uint32_t v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(acc[cc][j]);
+            store(v, cc);
+          }
+        }
       }
-      tc_fence_before();
-      mbar_arrive(&acc_empty[buf]);
-      ++unit;
     }
   }
 
   tc_fence_before();
   __syncwarp();
   __syncthreads();
+  if (kPair) pair_sync();  // neither SM leaves while the other may still signal or read it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, Shape::kTmem);
+    Tc::dealloc(tmem_base, Shape::kTmem);
   }
 }
 
 // the partial sums of a split reduction, added in order, and the epilogue
 template <typename T>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinProduct q) {
-  const long long words = q.ldp / 4, total = q.M * words;
+  const LinEpilogue e = q.e;
+  const long long words = q.ldp / 4, total = e.M * words, slab = e.M * q.ldp;
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total;
        i += static_cast<long long>(gridDim.x) * 256) {
     const long long row = i / words;
     const int c = static_cast<int>(i - row * words) * 4;
+    const float* from = q.partial + row * q.ldp + c;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < q.splits; ++s) {
-      const float4 f = *reinterpret_cast<const float4*>(q.partial + (static_cast<long long>(s) * q.M + row) * q.ldp + c);
+      const float4 f = *reinterpret_cast<const float4*>(from + s * slab);
       acc[0] += f.x; acc[1] += f.y; acc[2] += f.z; acc[3] += f.w;
     }
+    T* out = static_cast<T*>(e.out) + row * e.ldo + c;
+    T* pre = static_cast<T*>(e.pre) + row * e.ld_pre + c;
+    const T* from_res = static_cast<const T*>(e.residual) + row * e.ld_res + c;
+    const float bias[4] = {bias_at<T>(e, c), bias_at<T>(e, c + 1), bias_at<T>(e, c + 2), bias_at<T>(e, c + 3)};
+    Pack<T, 4> res, y, z;
+    const bool together = e.words && c + 4 <= e.N;  // four elements lie on a multiple of their size
+    if (e.residual) {
+      if (together) {
+        res = *reinterpret_cast<const Pack<T, 4>*>(from_res);
+      } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (c + j >= q.N) break;
-      float b[1], a[1] = {acc[j]};
-      load_bias<T, 1>(q, c + j, b);
-      Pack<T, 1> res;
-      res.v[0] = Elem<T>::narrow(0);
-      if (q.residual) res = load_residual<T, 1>(q, row, c + j);
-      finish_row<T, 1>(q, row, c + j, a, b, res);
+        for (int j = 0; j < 4; ++j) res.v[j] = c + j < e.N ? from_res[j] : Elem<T>::narrow(0);
+      }
+    }
+    finish_elements<T, 4>(e, acc, bias, res, y, z);
+    if (together) {
+      *reinterpret_cast<Pack<T, 4>*>(out) = y;
+      if (e.pre) *reinterpret_cast<Pack<T, 4>*>(pre) = z;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c + j >= e.N) break;
+        out[j] = y.v[j];
+        if (e.pre) pre[j] = z.v[j];
+      }
     }
   }
 }
@@ -448,21 +672,21 @@ __device__ __forceinline__ void split3(float v, __nv_bfloat16& a, __nv_bfloat16&
   b = __float2bfloat16_rn(r);
   c = __float2bfloat16_rn(r - __bfloat162float(b));
 }
-template <typename T> struct Plane { using type = T; static constexpr int kCount = 1; };
-template <> struct Plane<float> { using type = __nv_bfloat16; static constexpr int kCount = 3; };
-
 // eight consecutive results into the operand's planes
 template <typename T>
 __device__ __forceinline__ void store_planes(typename Plane<T>::type* dst, long long plane_stride, const float (&f)[8]) {
   using P = typename Plane<T>::type;
-  Pack<P, 8> p[Plane<T>::kCount];
+  if constexpr (Plane<T>::kCount == 3) {
+    Pack<P, 8> p[3];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if constexpr (Plane<T>::kCount == 3) split3(f[j], p[0].v[j], p[1].v[j], p[2].v[j]);
-    else p[0].v[j] = Elem<T>::narrow(f[j]);
+    for (int j = 0; j < 8; ++j) split3(f[j], p[0].v[j], p[1].v[j], p[2].v[j]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<Pack<P, 8>*>(dst + i * plane_stride) = p[i];
+  } else {
+    const Duo<float> d[4] = {Duo<float>::of(f[0], f[1]), Duo<float>::of(f[2], f[3]), Duo<float>::of(f[4], f[5]),
+                             Duo<float>::of(f[6], f[7])};
+    *reinterpret_cast<Word<P>*>(dst) = to_word<P>(d);
   }
-#pragma unroll
-  for (int i = 0; i < Plane<T>::kCount; ++i) *reinterpret_cast<Pack<P, 8>*>(dst + i * plane_stride) = p[i];
 }
 
 template <typename T, bool kWords>
@@ -471,9 +695,10 @@ __device__ __forceinline__ void load8(const T* row, int c, int n, float (&f)[8])
     constexpr int kV = kVec16<T>;
 #pragma unroll
     for (int i = 0; i < 8; i += kV) {
-      const Pack<T, kV> p = *reinterpret_cast<const Pack<T, kV>*>(row + c + i);
+      Duo<float> d[kDuos<T>];
+      widen_word(*reinterpret_cast<const Word<T>*>(row + c + i), d);
 #pragma unroll
-      for (int j = 0; j < kV; ++j) f[i + j] = Elem<T>::widen(p.v[j]);
+      for (int j = 0; j < kDuos<T>; ++j) { f[i + 2 * j] = d[j].lo(); f[i + 2 * j + 1] = d[j].hi(); }
     }
   } else {
 #pragma unroll
@@ -516,36 +741,79 @@ struct SlopeArgs {
   long long rows, ldg, ld_pre, ldd, plane_stride;
   int cols, act, words;
 };
+// act'(z) of a pair.  GELU, with s the logistic function of 2 u(z): s + s (1 - s) z 2 u'(z); z^2 is capped at
+// 10^6, where s is 0 or 1 for long, so that nothing overflows on the way.
+template <bool kExact> __device__ __forceinline__ Duo<float> slope_pair(Duo<float> z, int act) {
+  if (act == 1) return Duo<float>::of(z.lo() > 0.f ? 1.f : 0.f, z.hi() > 0.f ? 1.f : 0.f);
+  Duo<float> z2 = z * z;
+  z2 = Duo<float>::of(fminf(z2.lo(), 1e6f), fminf(z2.hi(), 1e6f));
+  const Duo<float> arg = z * fma2(both(2.f * kGeluA * kGeluB), z2, both(2.f * kGeluA));
+  const Duo<float> du = fma2(both(6.f * kGeluA * kGeluB), z2, both(2.f * kGeluA));
+  const Duo<float> s = Duo<float>::of(logistic<kExact>(arg.lo()), logistic<kExact>(arg.hi()));
+  const Duo<float> t = fma2(s * both(-1.f), s, s);  // s (1 - s)
+  return fma2(t * z, du, s);
+}
+
 // dz = grad_out act'(pre), rounded into the products' operand, and its column sums from the f32 values:
-// 256 columns per block, eight per lane; eight warps share the block's rows
+// 256 columns per block, eight per lane; eight warps share the block's rows, four (f32: two) rows on their way each
 template <typename T>
-__global__ void __launch_bounds__(256) linear_slope_kernel(const __grid_constant__ SlopeArgs a) {
+__global__ void __launch_bounds__(256, 3) linear_slope_kernel(const __grid_constant__ SlopeArgs a) {
   constexpr bool kExact = sizeof(T) == 4;
+  constexpr int kRows = sizeof(T) == 2 ? 4 : 2, kV = kVec16<T>, kD = kDuos<T>, kWords = 8 / kV;
   __shared__ float sm[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 256 + lane * 8;
-  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c < a.cols) {
-    for (long long r = static_cast<long long>(blockIdx.y) * 8 + warp; r < a.rows; r += static_cast<long long>(gridDim.y) * 8) {
-      float g[8], z[8];
-      const T* gr = static_cast<const T*>(a.grad_out) + r * a.ldg;
-      if (a.words) load8<T, true>(gr, c, a.cols, g);
-      else load8<T, false>(gr, c, a.cols, g);
-      if (a.act) {
-        const T* zr = static_cast<const T*>(a.pre) + r * a.ld_pre;
-        if (a.words) load8<T, true>(zr, c, a.cols, z);
-        else load8<T, false>(zr, c, a.cols, z);
+  const T zero = Elem<T>::narrow(0);
+  Duo<float> sum[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= activate_slope<kExact>(z[j], a.act);
+  for (int j = 0; j < 4; ++j) sum[j] = both(0.f);
+  if (c < a.cols) {
+    const long long step = static_cast<long long>(gridDim.y) * 8, first = static_cast<long long>(blockIdx.y) * 8 + warp;
+    const T* gr = static_cast<const T*>(a.grad_out) + first * a.ldg;
+    const T* zr = static_cast<const T*>(a.pre) + first * a.ld_pre;
+    typename Plane<T>::type* out = static_cast<typename Plane<T>::type*>(a.dz) + first * a.ldd + c;
+    for (long long r0 = first; r0 < a.rows; r0 += kRows * step) {
+      Word<T> g[kRows][kWords], z[kRows][kWords];
+#pragma unroll
+      for (int s = 0; s < kRows; ++s) {
+        if (r0 + s * step >= a.rows) break;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) g[s][w] = read_word(gr + s * step * a.ldg, c + w * kV, a.cols, a.words != 0, zero);
+        if (a.act) {
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) z[s][w] = read_word(zr + s * step * a.ld_pre, c + w * kV, a.cols, a.words != 0, zero);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] += g[j];
-      if (a.dz) store_planes<T>(static_cast<typename Plane<T>::type*>(a.dz) + r * a.ldd + c, a.plane_stride, g);
+      for (int s = 0; s < kRows; ++s) {
+        if (r0 + s * step >= a.rows) break;
+        Duo<float> d[4];
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          Duo<float> gw[kD], zw[kD];
+          widen_word(g[s][w], gw);
+          if (a.act) widen_word(z[s][w], zw);
+#pragma unroll
+          for (int j = 0; j < kD; ++j) d[w * kD + j] = a.act ? gw[j] * slope_pair<kExact>(zw[j], a.act) : gw[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = sum[j] + d[j];
+        if (a.dz) {
+          const float f[8] = {d[0].lo(), d[0].hi(), d[1].lo(), d[1].hi(), d[2].lo(), d[2].hi(), d[3].lo(), d[3].hi()};
+          store_planes<T>(out + s * step * a.ldd, a.plane_stride, f);
+        }
+      }
+      gr += kRows * step * a.ldg;
+      zr += kRows * step * a.ld_pre;
+      out += kRows * step * a.ldd;
     }
   }
   if (!a.partial) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sm[warp][lane * 8 + j] = sum[j];
+  for (int j = 0; j < 4; ++j) {
+    sm[warp][lane * 8 + 2 * j] = sum[j].lo();
+    sm[warp][lane * 8 + 2 * j + 1] = sum[j].hi();
+  }
   __syncthreads();
   const int col = blockIdx.x * 256 + threadIdx.x;
   float s = 0.f;
@@ -573,10 +841,6 @@ struct Stored {
   int planes;
 };
 
-int operand_map(CUtensorMap* map, const Stored& s, bool mn, int tile) {
-  return make_matrix_map16(map, s.p, s.inner, s.outer, s.ld, s.planes, s.plane_stride, mn ? 64 : tile);
-}
-
 bool tma_ready(const void* p, long long ld) { return rows_on_16_bytes<uint16_t>(p, ld); }
 
 struct ProductSpec {
@@ -585,108 +849,183 @@ struct ProductSpec {
   long long M, N, K;
 };
 
-template <int BN, typename T> int launch_products(const LinMaps& maps, const LinParams& prm, cudaStream_t st) {
-  const int sms = lib_num_sms();
-  linear_kernel<BN, T><<<prm.total_work < sms ? prm.total_work : sms, kLinThreads, LinShape<BN>::kSmem, st>>>(maps, prm);
+template <int BN, typename T, bool kPair>
+int launch_products(const ProductSpec* s, LinProduct* p, int n, LinParams& prm, cudaStream_t st) {
+  using Shape = LinShape<BN, T, kPair>;
+  LinMaps maps;
+  for (int i = 0; i < n; ++i) {
+    // K-major: a box of one k-block and the tile's rows; MN-major: 64 elements of the axis and one k-block
+    const Stored &a = s[i].a, &b = s[i].b;
+    if (make_matrix_map16(&maps.a[i], a.p, a.inner, a.outer, a.ld, a.planes, a.plane_stride, s[i].a_mn ? 64 : Shape::kBK,
+                          s[i].a_mn ? Shape::kBK : kLinBM) ||
+        make_matrix_map16(&maps.b[i], b.p, b.inner, b.outer, b.ld, b.planes, b.plane_stride, s[i].b_mn ? 64 : Shape::kBK,
+                          s[i].b_mn ? Shape::kBK : Shape::kBRows))
+      return -1;
+    prm.p[i] = p[i];
+  }
+  if (n == 1) { maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0]; }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(prm.workers) * (kPair ? 2u : 1u));
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = Shape::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kPair ? 2 : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_kernel<BN, T, kPair>, maps, prm);
+  if (e != cudaSuccess) {
+    fprintf(stderr, "[eshkol-b200] linear layer launch failed: %s\n", cudaGetErrorString(e));
+    cudaGetLastError();
+    return -1;
+  }
   return 1;
 }
 
 struct Plan {
-  int bn, splits[2], kb_per_split[2];
+  int bn;
+  bool pair;
+  int splits[2], kb_per_split[2];
   size_t partial_bytes[2];
+  double item_cost[2];
 };
 
-// Tile width and splits: the estimate of a launch in units of one k-block of a 128 x 256 tile.  An item
-// costs its k-blocks (a narrower tile's cost by the bytes it loads) and its epilogue; items run in rounds
-// over the SMs; a split product pays for its partial sums and the second launch.
-Plan plan_products(const ProductSpec* s, int n, int n_seg) {
-  const double sms = lib_num_sms();
+// Tile shape and splits, by an estimate in units of one k-block (64 elements) of a 128 x 256 tile, 0.28 us.
+// An item costs its k-blocks, the narrower its tile the more by what it loads, and a hand-over by its rows;
+// one product's items run in whole rounds over the workers, two products even each other out; a split
+// product pays for its partial sums and a second launch.  Measured at 8192 x 16384 x 4096 bf16: pairs of SMs
+// 725 us, single ones 778.
+template <typename T> Plan plan_products(const ProductSpec* s, int n) {
+  constexpr bool kSplit3 = Plane<T>::kCount == 3;
+  const int sms = lib_num_sms(), kbk = kSplit3 ? 32 : 64;
   Plan best = {};
   double best_cost = 1e300;
-  const int widths[3] = {256, 128, 64};
-  for (int bn : widths) {
-    const double per_kb = bn == 256 ? 1.0 : bn == 128 ? 0.62 : 0.46, per_tile = 4.0 * bn / 256 + 2.0;
+  // pairs on 256 x 256, single SMs on 128 x 256, 128 x 128, 128 x 64; f32: pairs on 256 x 128, then 128 x 128 and 128 x 64
+  for (int shape = 0; shape < 4; ++shape) {
+    if (kSplit3 && shape == 1) continue;
+    const int bn = kSplit3 ? (shape == 3 ? 64 : 128) : shape <= 1 ? 256 : shape == 2 ? 128 : 64;
     Plan q = {};
     q.bn = bn;
-    double items = 0, longest = 0, work = 0, extra = 0;
+    q.pair = shape == 0;
+    const int workers = q.pair ? sms / 2 : sms, bm = q.pair ? 256 : 128;
+    const double per_kb = kSplit3 ? (shape == 0 ? 2.3 : shape == 2 ? 2.9 : 1.8) : shape == 0 ? 0.93 : shape == 1 ? 1.0 : shape == 2 ? 0.6 : 0.42;
+    double longest = 0, work = 0, extra = 0, alone = 0;
     for (int i = 0; i < n; ++i) {
-      const double tiles = static_cast<double>((s[i].M + 127) / 128) * static_cast<double>((s[i].N + bn - 1) / bn);
-      const int kb = static_cast<int>((s[i].K + kLinBK - 1) / kLinBK) * n_seg;
-      int split = 1;
-      // enough items for the SMs, at least eight k-blocks in each
-      while (tiles * split < sms && kb / (split * 2) >= 8 && split < 64) split *= 2;
-      q.kb_per_split[i] = (kb + split - 1) / split;
-      q.splits[i] = (kb + q.kb_per_split[i] - 1) / q.kb_per_split[i];
-      const double cost = q.kb_per_split[i] * per_kb + per_tile;
-      items += tiles * q.splits[i];
-      work += tiles * q.splits[i] * cost;
-      if (cost > longest) longest = cost;
-      q.partial_bytes[i] = 0;
-      if (q.splits[i] > 1) {
-        q.partial_bytes[i] = (static_cast<size_t>(q.splits[i]) * s[i].M * ((s[i].N + 3) / 4 * 4) * 4 + 1023) & ~size_t(1023);
-        extra += 8.0 + q.partial_bytes[i] * 2.0 / 1.2e6;  // a k-block takes about 0.3 us
+      const double tiles = static_cast<double>((s[i].M + bm - 1) / bm) * static_cast<double>((s[i].N + bn - 1) / bn);
+      const int kb = static_cast<int>((s[i].K + kbk - 1) / kbk);
+      const double rows = s[i].M < bm ? static_cast<double>(s[i].M) : bm;
+      const double hand_over = 2.0 + 8.0 * bn / 256 * rows / bm;
+      double least = 1e300;
+      for (int split = 1; split <= 64 && (split == 1 || kb / split >= 2) && (split == 1 || tiles * (split - 1) < 8.0 * workers); ++split) {
+        int per = (kb + split - 1) / split;
+        if (kSplit3) per = (per + 7) / 8 * 8;  // whole hand-overs
+        const int parts = (kb + per - 1) / per;
+        const double item = (per < kb ? per : kb) * per_kb + hand_over;
+        const size_t bytes = parts > 1 ? (static_cast<size_t>(parts) * s[i].M * ((s[i].N + 3) / 4 * 4) * 4 + 1023) & ~size_t(1023) : 0;
+        const double join = parts > 1 ? 14.0 + bytes * 2.0 / 1.2e6 : 0.0;
+        const double cost = ceil(tiles * parts / workers) * item + join;
+        if (cost < least) {
+          least = cost;
+          q.kb_per_split[i] = per;
+          q.splits[i] = parts;
+          q.item_cost[i] = item;
+          q.partial_bytes[i] = bytes;
+          if (i == 0) { work = tiles * parts * item; longest = item; extra = join; alone = cost; }
+          else { alone = cost; }
+        }
+      }
+      if (i == 1) {
+        work += tiles * q.splits[1] * q.item_cost[1];
+        extra += q.partial_bytes[1] ? 14.0 + q.partial_bytes[1] * 2.0 / 1.2e6 : 0.0;
+        if (q.item_cost[1] > longest) longest = q.item_cost[1];
       }
     }
-    const double rounds = ceil(items / sms);
-    const double cost = fmax(work / sms, fmax(longest, rounds * work / items)) + extra;
+    const double cost = n == 1 ? alone : fmax(work / workers, longest) + extra;
     if (cost < best_cost) { best_cost = cost; best = q; }
   }
   return best;
 }
 
 // Multiplies one or two independent products in one launch, and joins those whose reduction was split.
-// epi[i] carries the epilogue of product i; scratch_at: room for the partial sums (plan.partial_bytes).
+// p[i].e carries the epilogue of product i; scratch_at: room for the partial sums (plan.partial_bytes).
 template <typename T>
-int run_products(const ProductSpec* s, LinProduct* epi, int n, const Plan& plan, uint8_t* scratch_at, cudaStream_t st) {
-  LinMaps maps;
+int run_products(const ProductSpec* s, LinProduct* p, int n, const Plan& plan, uint8_t* scratch_at, cudaStream_t st) {
+  constexpr int kBK = Plane<T>::kCount == 3 ? 32 : 64;
   LinParams prm;
   memset(&prm, 0, sizeof(prm));
-  static const int seg_a[6] = {2, 0, 1, 1, 0, 0}, seg_b[6] = {0, 2, 1, 0, 1, 0};
-  const int n_seg = Plane<T>::kCount == 3 ? 6 : 1;
+  const int bm = plan.pair ? 256 : kLinBM;
   long long total = 0;
   for (int i = 0; i < n; ++i) {
-    LinProduct& q = epi[i];
-    q.M = static_cast<int>(s[i].M);
-    q.N = static_cast<int>(s[i].N);
-    q.kb = static_cast<int>((s[i].K + kLinBK - 1) / kLinBK);
-    q.n_seg = n_seg;
-    for (int k = 0; k < n_seg; ++k) {
-      q.seg_a[k] = n_seg == 6 ? seg_a[k] : 0;
-      q.seg_b[k] = n_seg == 6 ? seg_b[k] : 0;
-    }
+    LinProduct& q = p[i];
+    q.e.M = static_cast<int>(s[i].M);
+    q.e.N = static_cast<int>(s[i].N);
+    q.kb = static_cast<int>((s[i].K + kBK - 1) / kBK);
     q.a_mn = s[i].a_mn; q.b_mn = s[i].b_mn;
-    q.tiles_m = (q.M + kLinBM - 1) / kLinBM;
-    q.tiles_n = (q.N + plan.bn - 1) / plan.bn;
+    q.tiles_m = (q.e.M + bm - 1) / bm;
+    q.tiles_n = (q.e.N + plan.bn - 1) / plan.bn;
     q.splits = plan.splits[i];
     q.kb_per_split = plan.kb_per_split[i];
-    q.first_work = static_cast<int>(total);
-    total += static_cast<long long>(q.tiles_m) * q.tiles_n * q.splits;
-    if (total > 0x7fffffffLL) return -1;
-    q.ldp = (q.N + 3) / 4 * 4;
+    const long long items = static_cast<long long>(q.tiles_m) * q.tiles_n * q.splits;
+    total += items;
+    if (total > 0x7fffffffLL - kMaxWorkers) return -1;
+    q.items = static_cast<int>(items);
+    q.ldp = (q.e.N + 3) / 4 * 4;
     q.partial = nullptr;
     if (q.splits > 1) {
       q.partial = reinterpret_cast<float*>(scratch_at);
       scratch_at += plan.partial_bytes[i];
     }
-    q.words = rows_on_16_bytes<T>(q.out, q.ldo) && (!q.pre || rows_on_16_bytes<T>(q.pre, q.ld_pre)) &&
-              (!q.residual || rows_on_16_bytes<T>(q.residual, q.ld_res));
-    if (operand_map(&maps.a[i], s[i].a, s[i].a_mn, kLinBM) || operand_map(&maps.b[i], s[i].b, s[i].b_mn, plan.bn)) return -1;
-    prm.p[i] = q;
+    q.e.words = rows_on_16_bytes<T>(q.e.out, q.e.ldo) && (!q.e.pre || rows_on_16_bytes<T>(q.e.pre, q.e.ld_pre)) &&
+                (!q.e.residual || rows_on_16_bytes<T>(q.e.residual, q.e.ld_res));
   }
-  if (n == 1) { maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0]; }
+  // workers: no more than items, and no more than `start` has room for
+  int workers = lib_num_sms();
+  if (workers > kMaxWorkers) workers = kMaxWorkers;
+  if (plan.pair) workers /= 2;
+  if (total < workers) workers = static_cast<int>(total);
   prm.n_products = n;
-  prm.total_work = static_cast<int>(total);
-  prm.formats = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? 0u : (1u << 7) | (1u << 10);
+  prm.workers = workers;
+  if (n == 2) {
+    // shares of the second product: what every worker lacks to the level of all
+    const double c0 = plan.item_cost[0], c1 = plan.item_cost[1];
+    double level = (c0 * p[0].items + c1 * p[1].items) / workers, sum = 0, lack[kMaxWorkers];
+    for (int w = 0; w < workers; ++w) {
+      const int mine = p[0].items / workers + (w < p[0].items % workers ? 1 : 0);
+      lack[w] = fmax(0.0, level - c0 * mine);
+      sum += lack[w];
+    }
+    double before = 0;
+    for (int w = 0; w < workers; ++w) {
+      prm.start[w] = sum > 0 ? static_cast<int>(floor(before / sum * p[1].items + 0.5))
+                             : static_cast<int>(static_cast<long long>(p[1].items) * w / workers);
+      before += lack[w];
+    }
+    prm.start[0] = 0;
+    prm.start[workers] = p[1].items;
+  }
+  prm.formats = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
   prm.status = lib_status_word();
   prm.wait_ns = lib_wait_limit_ns();
   prm.withhold = lib_take_withhold();
-  int launches = plan.bn == 256 ? launch_products<256, T>(maps, prm, st)
-                 : plan.bn == 128 ? launch_products<128, T>(maps, prm, st) : launch_products<64, T>(maps, prm, st);
+  int launches = -1;
+  if constexpr (Plane<T>::kCount == 3) {
+    launches = plan.pair       ? launch_products<128, T, true>(s, p, n, prm, st)
+               : plan.bn == 128 ? launch_products<128, T, false>(s, p, n, prm, st)
+                                : launch_products<64, T, false>(s, p, n, prm, st);
+  } else {
+    launches = plan.pair        ? launch_products<256, T, true>(s, p, n, prm, st)
+               : plan.bn == 256 ? launch_products<256, T, false>(s, p, n, prm, st)
+               : plan.bn == 128 ? launch_products<128, T, false>(s, p, n, prm, st)
+                                : launch_products<64, T, false>(s, p, n, prm, st);
+  }
+  if (launches < 0) return -1;
   for (int i = 0; i < n; ++i) {
-    if (epi[i].splits == 1) continue;
-    const long long words = epi[i].ldp / 4 * epi[i].M, cap = static_cast<long long>(lib_num_sms()) * 8;
+    if (p[i].splits == 1) continue;
+    const long long words = p[i].ldp / 4 * p[i].e.M, cap = static_cast<long long>(lib_num_sms()) * 8;
     const long long blocks = (words + 255) / 256;
-    linear_join_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, st>>>(epi[i]);
+    linear_join_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, st>>>(p[i]);
     ++launches;
   }
   return launches;
@@ -759,7 +1098,7 @@ template <typename T> int linear_forward(const LinearArgs& a, void* y, OpScratch
   Operand<T> x(a.x, a.rows, a.d_in, a.ldx, false, cv);
   Operand<T> w(a.w, tw ? a.d_out : a.d_in, tw ? a.d_in : a.d_out, a.ldw, false, cv);
   ProductSpec s = {x.s, w.s, false, !tw, a.rows, a.d_out, a.d_in};
-  const Plan plan = plan_products(&s, 1, Plane<T>::kCount == 3 ? 6 : 1);
+  const Plan plan = plan_products<T>(&s, 1);
   const size_t parts = cv.take(plan.partial_bytes[0]);
   uint8_t* base = scratch.reserve(cv.off, st);
   if (!base) return -1;
@@ -772,8 +1111,8 @@ template <typename T> int linear_forward(const LinearArgs& a, void* y, OpScratch
   const int packs = launch_pack<T>(jobs, st);
   LinProduct epi;
   memset(&epi, 0, sizeof(epi));
-  epi.bias = a.o.bias; epi.residual = a.o.residual; epi.out = y; epi.pre = a.o.pre;
-  epi.ldo = a.ldy; epi.ld_res = a.ld_res; epi.ld_pre = a.ld_pre; epi.act = a.o.activation;
+  epi.e.bias = a.o.bias; epi.e.residual = a.o.residual; epi.e.out = y; epi.e.pre = a.o.pre;
+  epi.e.ldo = a.ldy; epi.e.ld_res = a.ld_res; epi.e.ld_pre = a.ld_pre; epi.e.act = a.o.activation;
   const int n = run_products<T>(&s, &epi, 1, plan, base + parts, st);
   return n < 0 ? -1 : packs + n;
 }
@@ -795,23 +1134,23 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
     n = 0;
     if (grad_x) {
       s[n] = {dz.s, w.s, false, tw, a.rows, a.d_in, a.d_out};
-      epi[n].out = grad_x; epi[n].ldo = a.ldx;
+      epi[n].e.out = grad_x; epi[n].e.ldo = a.ldx;
       ++n;
     }
     if (grad_w) {
       if (tw) s[n] = {dz.s, x.s, true, true, a.d_out, a.d_in, a.rows};
       else s[n] = {x.s, dz.s, true, true, a.d_in, a.d_out, a.rows};
-      epi[n].out = grad_w; epi[n].ldo = a.ldw;
+      epi[n].e.out = grad_w; epi[n].e.ldo = a.ldw;
       ++n;
     }
   };
   describe();
   Plan plan = {};
-  if (n) plan = plan_products(s, n, Plane<T>::kCount == 3 ? 6 : 1);
+  if (n) plan = plan_products<T>(s, n);
   const size_t parts = cv.take(plan.partial_bytes[0] + plan.partial_bytes[1]);
-  // blocks of the column sums: the SMs several times over, at least 16 rows a block
+  // blocks: as many as the SMs hold at once, at least 16 rows in each
   const long long col_blocks = (a.d_out + 255) / 256;
-  long long row_blocks = static_cast<long long>(lib_num_sms()) * 6 / col_blocks;
+  long long row_blocks = static_cast<long long>(lib_num_sms()) * 3 / col_blocks;
   if (row_blocks > (a.rows + 15) / 16) row_blocks = (a.rows + 15) / 16;
   if (row_blocks < 1) row_blocks = 1;
   const size_t sums = cv.take(grad_bias ? static_cast<size_t>(row_blocks) * a.d_out * 4 : 0);
@@ -827,7 +1166,8 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
     q.rows = a.rows; q.ldg = a.ldy; q.ld_pre = a.ld_pre; q.ldd = dz.s.ld; q.plane_stride = dz.s.plane_stride;
     q.cols = static_cast<int>(a.d_out); q.act = a.o.activation;
     q.words = rows_on_16_bytes<T>(grad_out, a.ldy) && (!q.act || rows_on_16_bytes<T>(q.pre, a.ld_pre));
-    linear_slope_kernel<T><<<dim3(static_cast<unsigned>(col_blocks), static_cast<unsigned>(row_blocks)), 256, 0, st>>>(q);
+    const dim3 grid(static_cast<unsigned>(col_blocks), static_cast<unsigned>(row_blocks));
+    linear_slope_kernel<T><<<grid, 256, 0, st>>>(q);
     ++launches;
     if (grad_bias) {
       linear_bias_join_kernel<<<static_cast<unsigned>(col_blocks), 256, 0, st>>>(
@@ -870,14 +1210,19 @@ int check(const EshkolB200LinearOpts* opts, uint64_t rows, uint64_t d_in, uint64
   return 0;
 }
 
-template <int BN, typename T> cudaError_t set_attribute() {
-  return cudaFuncSetAttribute(linear_kernel<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(LinShape<BN>::kSmem));
+template <int BN, typename T, bool kPair> cudaError_t set_attribute() {
+  return cudaFuncSetAttribute(linear_kernel<BN, T, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(LinShape<BN, T, kPair>::kSmem));
 }
 template <typename T> cudaError_t set_attributes_of() {
-  cudaError_t e = set_attribute<256, T>();
-  if (e == cudaSuccess) e = set_attribute<128, T>();
-  if (e == cudaSuccess) e = set_attribute<64, T>();
+  cudaError_t e = set_attribute<128, T, false>();
+  if (e == cudaSuccess) e = set_attribute<64, T, false>();
+  if constexpr (Plane<T>::kCount == 1) {
+    if (e == cudaSuccess) e = set_attribute<256, T, false>();
+    if (e == cudaSuccess) e = set_attribute<256, T, true>();
+  } else {
+    if (e == cudaSuccess) e = set_attribute<128, T, true>();
+  }
   return e;
 }
 

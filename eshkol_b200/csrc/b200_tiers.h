@@ -21,9 +21,10 @@ void count_launches(int n);
 int make_plane_map(CUtensorMap* map, const void* base, long long inner_bytes, long long rows,
                    long long planes, long long plane_stride, int box_rows);
 // a row-major matrix of 16-bit elements (`inner` in a row, pitch `ld`), `planes` of them plane_stride
-// elements apart, tiled {64 elements, box_rows, 1} with the 128-byte swizzle; zero beyond its extent
+// elements apart, tiled {box_inner, box_rows, 1} with the swizzle of a row of box_inner elements (64: 128
+// bytes, 32: 64 bytes); zero beyond its extent
 int make_matrix_map16(CUtensorMap* map, const void* base, long long inner, long long rows, long long ld,
-                      long long planes, long long plane_stride, int box_rows);
+                      long long planes, long long plane_stride, int box_inner, int box_rows);
 void oz2_host_consts(int n_mod, Oz2DeviceConsts* c, double* log2P);
 int ozaki2_exact_gemm_im2col(const double* dA, const Im2colView& view, double* dC, long long M, long long K,
                              long long N, const EshkolB200GemmOpts& o);
