@@ -36,7 +36,6 @@ constexpr int kLinUmmaK = 16;
 constexpr int kStagePitch = 36;     // f32 per row of a warp's 16 x 32 exchange tile: 16-byte accesses without conflicts
 constexpr int kExchange = 16 * kStagePitch + 128;  // f32 of an epilogue warp: the exchange tile, its columns' bias
 constexpr uint32_t kExchangeBytes = 8 * kExchange * 4;
-constexpr int kMaxWorkers = 160;
 
 // 16-bit operands as they are, f32 as three bf16 planes
 template <typename T> struct Plane { using type = T; static constexpr int kCount = 1; };
@@ -81,12 +80,13 @@ struct LinProduct {
   long long ldp;
 };
 
-// The workers (SMs, or pairs) take the first product's items in turn, and then of the second product's
-// items each a share that evens out their work.
+// The workers (SMs, or pairs) take the first product's items in turn, then the second's.  Where the first
+// product leaves some workers, the first `late` of them, with one item more, the others take `head` items of
+// the second product meanwhile.  In every round the workers are at neighbouring tiles, whose operands L2
+// then serves to many.
 struct LinParams {
   LinProduct p[2];
-  int n_products, workers;
-  int start[kMaxWorkers + 1];  // of the shares
+  int n_products, workers, late, head;
   uint32_t formats;       // operand type bits of the instruction descriptor
   int* status;
   unsigned long long wait_ns;
@@ -102,23 +102,22 @@ struct LinWork {
 };
 // a worker's way through its items, the same for all its warps
 struct LinSchedule {
-  int at0, step, end0, at1, end1;
-  __device__ __forceinline__ LinSchedule(const LinParams& prm, int worker) {
-    at0 = worker;
-    step = prm.workers;
-    end0 = prm.p[0].items;
-    at1 = prm.n_products > 1 ? prm.start[worker] : 0;
-    end1 = prm.n_products > 1 ? prm.start[worker + 1] : 0;
-  }
+  int at0, step, worker, round1;
+  __device__ __forceinline__ LinSchedule(const LinParams& prm, int w) : at0(w), step(prm.workers), worker(w), round1(0) {}
   __device__ __forceinline__ bool next(const LinParams& prm, LinWork& it) {
     int t;
-    if (at0 < end0) {
+    if (at0 < prm.p[0].items) {
       it.which = 0;
       t = at0;
       at0 += step;
-    } else if (at1 < end1) {
+    } else if (prm.n_products > 1) {
+      const int early = step - prm.late, ahead = prm.head * early;
+      if (worker < prm.late) t = ahead + round1 * step + worker;
+      else if (round1 < prm.head) t = round1 * early + worker - prm.late;
+      else t = ahead + (round1 - prm.head) * step + worker;
+      ++round1;
+      if (t >= prm.p[1].items) return false;
       it.which = 1;
-      t = at1++;
     } else {
       return false;
     }
@@ -755,11 +754,14 @@ template <bool kExact> __device__ __forceinline__ Duo<float> slope_pair(Duo<floa
 }
 
 // dz = grad_out act'(pre), rounded into the products' operand, and its column sums from the f32 values:
-// 256 columns per block, eight per lane; eight warps share the block's rows, four (f32: two) rows on their way each
-template <typename T>
-__global__ void __launch_bounds__(256, 3) linear_slope_kernel(const __grid_constant__ SlopeArgs a) {
+// 256 columns per block, eight per lane; eight warps share the block's rows, the next kDepth of each on their
+// way in shared memory
+constexpr int kSlopeDepth = 4;
+template <typename T, int kHow>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) linear_slope_kernel(const __grid_constant__ SlopeArgs a) {
   constexpr bool kExact = sizeof(T) == 4;
-  constexpr int kRows = sizeof(T) == 2 ? 4 : 2, kV = kVec16<T>, kD = kDuos<T>, kWords = 8 / kV;
+  constexpr int kV = kVec16<T>, kD = kDuos<T>, kWords = 8 / kV;
+  extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ float sm[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 256 + lane * 8;
@@ -770,43 +772,69 @@ __global__ void __launch_bounds__(256, 3) linear_slope_kernel(const __grid_const
   if (c < a.cols) {
     const long long step = static_cast<long long>(gridDim.y) * 8, first = static_cast<long long>(blockIdx.y) * 8 + warp;
     const T* gr = static_cast<const T*>(a.grad_out) + first * a.ldg;
-    const T* zr = static_cast<const T*>(a.pre) + first * a.ld_pre;
+    const T* zr = a.act ? static_cast<const T*>(a.pre) + first * a.ld_pre : nullptr;
     typename Plane<T>::type* out = static_cast<typename Plane<T>::type*>(a.dz) + first * a.ldd + c;
-    for (long long r0 = first; r0 < a.rows; r0 += kRows * step) {
-      Word<T> g[kRows][kWords], z[kRows][kWords];
+    const long long g_step = step * a.ldg, z_step = step * a.ld_pre, out_step = step * a.ldd;
+    long long coming = first;
+    Word<T>* ring = reinterpret_cast<Word<T>*>(dyn) + threadIdx.x;  // [stage][grad_out or pre][word][thread]
+    const auto fetch = [&](int stage) {
+      if constexpr (kHow != kInRegisters) {
+        if (coming < a.rows) {
 #pragma unroll
-      for (int s = 0; s < kRows; ++s) {
-        if (r0 + s * step >= a.rows) break;
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) g[s][w] = read_word(gr + s * step * a.ldg, c + w * kV, a.cols, a.words != 0, zero);
-        if (a.act) {
-#pragma unroll
-          for (int w = 0; w < kWords; ++w) z[s][w] = read_word(zr + s * step * a.ld_pre, c + w * kV, a.cols, a.words != 0, zero);
+          for (int w = 0; w < kWords; ++w) {
+            if (kHow == kByWords || c + w * kV < a.cols) {
+              copy_word<T, kHow>(ring + ((stage * 2) * kWords + w) * 256, gr, c + w * kV, a.cols);
+              if (a.act) copy_word<T, kHow>(ring + ((stage * 2 + 1) * kWords + w) * 256, zr, c + w * kV, a.cols);
+            }
+          }
         }
+        commit_async();
+        coming += step;
+        gr += g_step;
+        zr += z_step;
       }
+    };
 #pragma unroll
-      for (int s = 0; s < kRows; ++s) {
-        if (r0 + s * step >= a.rows) break;
-        Duo<float> d[4];
+    for (int s = 0; s < kSlopeDepth; ++s) fetch(s);
+    int stage = 0;
+    for (long long r = first; r < a.rows; r += step) {
+      Word<T> g[kWords], z[kWords];
+      if constexpr (kHow != kInRegisters) {
+        wait_async<kSlopeDepth - 1>();
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-          Duo<float> gw[kD], zw[kD];
-          widen_word(g[s][w], gw);
-          if (a.act) widen_word(z[s][w], zw);
-#pragma unroll
-          for (int j = 0; j < kD; ++j) d[w * kD + j] = a.act ? gw[j] * slope_pair<kExact>(zw[j], a.act) : gw[j];
+          g[w] = take_word<T, kHow>(ring + ((stage * 2) * kWords + w) * 256, c + w * kV, a.cols, zero);
+          if (a.act) z[w] = take_word<T, kHow>(ring + ((stage * 2 + 1) * kWords + w) * 256, c + w * kV, a.cols, zero);
         }
+        fetch(stage);
+        stage = stage + 1 == kSlopeDepth ? 0 : stage + 1;
+      } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] = sum[j] + d[j];
-        if (a.dz) {
-          const float f[8] = {d[0].lo(), d[0].hi(), d[1].lo(), d[1].hi(), d[2].lo(), d[2].hi(), d[3].lo(), d[3].hi()};
-          store_planes<T>(out + s * step * a.ldd, a.plane_stride, f);
+        for (int w = 0; w < kWords; ++w) {
+          g[w] = read_word(gr, c + w * kV, a.cols, false, zero);
+          if (a.act) z[w] = read_word(zr, c + w * kV, a.cols, false, zero);
         }
+        gr += g_step;
+        zr += z_step;
       }
-      gr += kRows * step * a.ldg;
-      zr += kRows * step * a.ld_pre;
-      out += kRows * step * a.ldd;
+      Duo<float> d[4];
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        Duo<float> gw[kD], zw[kD];
+        widen_word(g[w], gw);
+        if (a.act) widen_word(z[w], zw);
+#pragma unroll
+        for (int j = 0; j < kD; ++j) d[w * kD + j] = a.act ? gw[j] * slope_pair<kExact>(zw[j], a.act) : gw[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = sum[j] + d[j];
+      if (a.dz) {
+        const float f[8] = {d[0].lo(), d[0].hi(), d[1].lo(), d[1].hi(), d[2].lo(), d[2].hi(), d[3].lo(), d[3].hi()};
+        store_planes<T>(out, a.plane_stride, f);
+      }
+      out += out_step;
     }
+    if constexpr (kHow != kInRegisters) wait_async<0>();
   }
   if (!a.partial) return;
 #pragma unroll
@@ -969,7 +997,7 @@ int run_products(const ProductSpec* s, LinProduct* p, int n, const Plan& plan, u
     q.kb_per_split = plan.kb_per_split[i];
     const long long items = static_cast<long long>(q.tiles_m) * q.tiles_n * q.splits;
     total += items;
-    if (total > 0x7fffffffLL - kMaxWorkers) return -1;
+    if (total > 0x3fffffffLL) return -1;
     q.items = static_cast<int>(items);
     q.ldp = (q.e.N + 3) / 4 * 4;
     q.partial = nullptr;
@@ -980,30 +1008,16 @@ int run_products(const ProductSpec* s, LinProduct* p, int n, const Plan& plan, u
     q.e.words = rows_on_16_bytes<T>(q.e.out, q.e.ldo) && (!q.e.pre || rows_on_16_bytes<T>(q.e.pre, q.e.ld_pre)) &&
                 (!q.e.residual || rows_on_16_bytes<T>(q.e.residual, q.e.ld_res));
   }
-  // workers: no more than items, and no more than `start` has room for
   int workers = lib_num_sms();
-  if (workers > kMaxWorkers) workers = kMaxWorkers;
   if (plan.pair) workers /= 2;
   if (total < workers) workers = static_cast<int>(total);
   prm.n_products = n;
   prm.workers = workers;
   if (n == 2) {
-    // shares of the second product: what every worker lacks to the level of all
-    const double c0 = plan.item_cost[0], c1 = plan.item_cost[1];
-    double level = (c0 * p[0].items + c1 * p[1].items) / workers, sum = 0, lack[kMaxWorkers];
-    for (int w = 0; w < workers; ++w) {
-      const int mine = p[0].items / workers + (w < p[0].items % workers ? 1 : 0);
-      lack[w] = fmax(0.0, level - c0 * mine);
-      sum += lack[w];
-    }
-    double before = 0;
-    for (int w = 0; w < workers; ++w) {
-      prm.start[w] = sum > 0 ? static_cast<int>(floor(before / sum * p[1].items + 0.5))
-                             : static_cast<int>(static_cast<long long>(p[1].items) * w / workers);
-      before += lack[w];
-    }
-    prm.start[0] = 0;
-    prm.start[workers] = p[1].items;
+    prm.late = p[0].items % workers;
+    prm.head = prm.late ? static_cast<int>(floor(plan.item_cost[0] / plan.item_cost[1] + 0.5)) : 0;
+    // no more ahead than there are
+    while (prm.head > 0 && static_cast<long long>(prm.head) * (workers - prm.late) > p[1].items) --prm.head;
   }
   prm.formats = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
   prm.status = lib_status_word();
@@ -1150,7 +1164,7 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
   const size_t parts = cv.take(plan.partial_bytes[0] + plan.partial_bytes[1]);
   // blocks: as many as the SMs hold at once, at least 16 rows in each
   const long long col_blocks = (a.d_out + 255) / 256;
-  long long row_blocks = static_cast<long long>(lib_num_sms()) * 3 / col_blocks;
+  long long row_blocks = static_cast<long long>(lib_num_sms()) * (sizeof(T) == 2 ? 4 : 3) / col_blocks;
   if (row_blocks > (a.rows + 15) / 16) row_blocks = (a.rows + 15) / 16;
   if (row_blocks < 1) row_blocks = 1;
   const size_t sums = cv.take(grad_bias ? static_cast<size_t>(row_blocks) * a.d_out * 4 : 0);
@@ -1167,7 +1181,10 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
     q.cols = static_cast<int>(a.d_out); q.act = a.o.activation;
     q.words = rows_on_16_bytes<T>(grad_out, a.ldy) && (!q.act || rows_on_16_bytes<T>(q.pre, a.ld_pre));
     const dim3 grid(static_cast<unsigned>(col_blocks), static_cast<unsigned>(row_blocks));
-    linear_slope_kernel<T><<<grid, 256, 0, st>>>(q);
+    constexpr int kWhole = kByWords, kParts = sizeof(T) >= 4 ? kByElements : kInRegisters;
+    constexpr size_t smem = static_cast<size_t>(kSlopeDepth) * 2 * (8 / kVec16<T>) * 256 * 16;
+    if (q.words && a.d_out % 8 == 0) linear_slope_kernel<T, kWhole><<<grid, 256, smem, st>>>(q);
+    else linear_slope_kernel<T, kParts><<<grid, 256, kParts == kInRegisters ? 0 : smem, st>>>(q);
     ++launches;
     if (grad_bias) {
       linear_bias_join_kernel<<<static_cast<unsigned>(col_blocks), 256, 0, st>>>(
@@ -1215,7 +1232,13 @@ template <int BN, typename T, bool kPair> cudaError_t set_attribute() {
                               static_cast<int>(LinShape<BN, T, kPair>::kSmem));
 }
 template <typename T> cudaError_t set_attributes_of() {
-  cudaError_t e = set_attribute<128, T, false>();
+  constexpr int kSlopeBytes = kSlopeDepth * 2 * (8 / kVec16<T>) * 256 * 16;
+  cudaError_t e = cudaFuncSetAttribute(linear_slope_kernel<T, kByWords>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlopeBytes);
+  if constexpr (sizeof(T) >= 4) {
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(linear_slope_kernel<T, kByElements>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlopeBytes);
+  }
+  if (e == cudaSuccess) e = set_attribute<128, T, false>();
   if (e == cudaSuccess) e = set_attribute<64, T, false>();
   if constexpr (Plane<T>::kCount == 1) {
     if (e == cudaSuccess) e = set_attribute<256, T, false>();
