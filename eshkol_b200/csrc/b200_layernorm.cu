@@ -145,9 +145,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 25
       if (beta) widen_word(get_word<T, kHow>(beta, c, n, a.beta_words, zero), b);
 #pragma unroll
       for (int j = 0; j < kD; ++j) {
-        const D xhat = (d[i][j] + both(-off)) * both(r_std);
-        const D scaled = gamma ? xhat * g[j] : xhat;
-        d[i][j] = beta ? scaled + b[j] : scaled;
+        const D scale = gamma ? g[j] * both(r_std) : both(r_std), centred = d[i][j] + both(-off);
+        d[i][j] = beta ? fma2(centred, scale, b[j]) : centred * scale;
       }
       put_word<T, kHow>(out, c, n, a.y_words, to_word<T>(d[i]));
     }

@@ -14,7 +14,7 @@
 // but for the last rounding, relative 2^-27), and six of the nine products of the parts make the result;
 // the three left out are below 2^-26 of the terms.
 //
-// Few output tiles and a long reduction: the reduction is split over blocks, their f32 sums go to scratch
+// A few rows: b200_linear_small.cu.  Few output tiles and a long reduction: the reduction is split over blocks, their f32 sums go to scratch
 // and a second kernel adds them in order and applies the epilogue.
 #include <math.h>
 #include <stdio.h>
@@ -25,6 +25,7 @@
 #include "b200_common.cuh"
 #include "b200_elem.cuh"
 #include "b200_internal.h"
+#include "b200_linear.cuh"
 #include "b200_tiers.h"
 
 namespace b200 {
@@ -59,15 +60,6 @@ template <int BN, typename T, bool kPair> struct LinShape {
   static constexpr int kStages = 196608 / kStageBytes;
   static constexpr uint32_t kTmem = 2 * kAccs * BN;
   static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kExchangeBytes + 1024;
-};
-
-// What becomes of a product's sums
-struct LinEpilogue {
-  const void *bias, *residual;
-  void *out, *pre;
-  long long ldo, ld_res, ld_pre;
-  int M, N, act;
-  int words;              // 1: out, pre and residual rows lie on 16-byte boundaries
 };
 
 // One product C[M x N] = A B
@@ -217,46 +209,6 @@ template <> struct Tensor<true> {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_address(smem_u32(bar))) : "memory");
   }
 };
-
-// ------------------------------------------------------------------ activations
-// Roundings are written out (no contraction left to the compiler), so that a result does not depend on
-// which other results a call asks for.
-template <bool kExact> __device__ __forceinline__ float logistic(float v) {
-  if (kExact) return __fdiv_rn(1.f, __fadd_rn(1.f, expf(-v)));
-  // a few 2^-22: below half a step of the 16-bit results
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(v, -1.4426950408889634f)));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.f, e)));
-  return r;
-}
-constexpr float kGeluA = 0.7978845608028654f, kGeluB = 0.044715f;
-// 2 u(z) = 2 A (z + B z^3)
-__device__ __forceinline__ float gelu_argument(float z) {
-  return __fmul_rn(z, __fmaf_rn(2.f * kGeluA * kGeluB, __fmul_rn(z, z), 2.f * kGeluA));
-}
-// 0 none, 1 ReLU, 2 the tanh form of GELU: z (1 + tanh u) / 2 = z logistic(2 u)
-template <bool kExact> __device__ __forceinline__ float activate(float z, int act) {
-  if (act == 1) return z > 0.f ? z : 0.f;
-  if (act == 2) return __fmul_rn(z, logistic<kExact>(gelu_argument(z)));
-  return z;
-}
-// kV elements of a row: bias, activation, residual, the two results
-template <typename T, int kV>
-__device__ __forceinline__ void finish_elements(const LinEpilogue& e, const float (&acc)[kV], const float (&bias)[kV],
-                                                const Pack<T, kV>& res, Pack<T, kV>& y, Pack<T, kV>& pre) {
-  constexpr bool kExact = sizeof(T) == 4;
-#pragma unroll
-  for (int j = 0; j < kV; ++j) {
-    const float z = __fadd_rn(acc[j], bias[j]);
-    float a = activate<kExact>(z, e.act);
-    if (e.residual) a = __fadd_rn(a, Elem<T>::widen(res.v[j]));
-    pre.v[j] = Elem<T>::narrow(z);
-    y.v[j] = Elem<T>::narrow(a);
-  }
-}
-template <typename T> __device__ __forceinline__ float bias_at(const LinEpilogue& e, int c) {
-  return (e.bias && c < e.N) ? Elem<T>::widen(static_cast<const T*>(e.bias)[c]) : 0.f;
-}
 
 // A 32 x 32 block of sums, one row per lane in v.  Where rows lie on 16-byte boundaries a lane writes its own
 // row's 64 (f32: 128) bytes: whole sectors, and nothing to exchange.
@@ -740,19 +692,6 @@ struct SlopeArgs {
   long long rows, ldg, ld_pre, ldd, plane_stride;
   int cols, act, words;
 };
-// act'(z) of a pair.  GELU, with s the logistic function of 2 u(z): s + s (1 - s) z 2 u'(z); z^2 is capped at
-// 10^6, where s is 0 or 1 for long, so that nothing overflows on the way.
-template <bool kExact> __device__ __forceinline__ Duo<float> slope_pair(Duo<float> z, int act) {
-  if (act == 1) return Duo<float>::of(z.lo() > 0.f ? 1.f : 0.f, z.hi() > 0.f ? 1.f : 0.f);
-  Duo<float> z2 = z * z;
-  z2 = Duo<float>::of(fminf(z2.lo(), 1e6f), fminf(z2.hi(), 1e6f));
-  const Duo<float> arg = z * fma2(both(2.f * kGeluA * kGeluB), z2, both(2.f * kGeluA));
-  const Duo<float> du = fma2(both(6.f * kGeluA * kGeluB), z2, both(2.f * kGeluA));
-  const Duo<float> s = Duo<float>::of(logistic<kExact>(arg.lo()), logistic<kExact>(arg.hi()));
-  const Duo<float> t = fma2(s * both(-1.f), s, s);  // s (1 - s)
-  return fma2(t * z, du, s);
-}
-
 // dz = grad_out act'(pre), rounded into the products' operand, and its column sums from the f32 values:
 // 256 columns per block, eight per lane; eight warps share the block's rows, the next kDepth of each on their
 // way in shared memory
@@ -1108,6 +1047,18 @@ struct LinearArgs {
 
 template <typename T> int linear_forward(const LinearArgs& a, void* y, OpScratch& scratch, cudaStream_t st) {
   const bool tw = a.o.trans_w != 0;
+  LinProduct epi;
+  memset(&epi, 0, sizeof(epi));
+  epi.e.bias = a.o.bias; epi.e.residual = a.o.residual; epi.e.out = y; epi.e.pre = a.o.pre;
+  epi.e.ldo = a.ldy; epi.e.ld_res = a.ld_res; epi.e.ld_pre = a.ld_pre; epi.e.act = a.o.activation;
+  if (few_rows<T>(a.rows, a.w, a.ldw, tw)) {
+    SmallRows q;
+    memset(&q, 0, sizeof(q));
+    q.e = epi.e;
+    q.e.M = static_cast<int>(a.rows); q.e.N = static_cast<int>(a.d_out);
+    q.a = a.x; q.lda = a.ldx; q.w = a.w; q.ldw = a.ldw; q.K = a.d_in; q.k_contiguous = tw;
+    return launch_small_rows<T>(q, st);
+  }
   Carver cv;
   Operand<T> x(a.x, a.rows, a.d_in, a.ldx, false, cv);
   Operand<T> w(a.w, tw ? a.d_out : a.d_in, tw ? a.d_in : a.d_out, a.ldw, false, cv);
@@ -1123,10 +1074,6 @@ template <typename T> int linear_forward(const LinearArgs& a, void* y, OpScratch
   add_pack<T>(jobs, a.x, a.ldx, x);
   add_pack<T>(jobs, a.w, a.ldw, w);
   const int packs = launch_pack<T>(jobs, st);
-  LinProduct epi;
-  memset(&epi, 0, sizeof(epi));
-  epi.e.bias = a.o.bias; epi.e.residual = a.o.residual; epi.e.out = y; epi.e.pre = a.o.pre;
-  epi.e.ldo = a.ldy; epi.e.ld_res = a.ld_res; epi.e.ld_pre = a.ld_pre; epi.e.act = a.o.activation;
   const int n = run_products<T>(&s, &epi, 1, plan, base + parts, st);
   return n < 0 ? -1 : packs + n;
 }
@@ -1134,12 +1081,27 @@ template <typename T> int linear_forward(const LinearArgs& a, void* y, OpScratch
 template <typename T>
 int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, void* grad_w, void* grad_bias,
                      OpScratch& scratch, cudaStream_t st) {
-  const bool tw = a.o.trans_w != 0, products = grad_x || grad_w;
+  const bool tw = a.o.trans_w != 0;
+  int launches = 0;
+  if (grad_x && few_rows<T>(a.rows, a.w, a.ldw, !tw)) {  // dz as it is needed, from grad_out and pre
+    SmallRows q;
+    memset(&q, 0, sizeof(q));
+    q.e.out = grad_x; q.e.ldo = a.ldx;
+    q.e.M = static_cast<int>(a.rows); q.e.N = static_cast<int>(a.d_in);
+    q.a = grad_out; q.lda = a.ldy; q.pre = a.o.pre; q.ld_pre = a.ld_pre; q.slope = a.o.activation;
+    q.w = a.w; q.ldw = a.ldw; q.K = a.d_out; q.k_contiguous = !tw;
+    launches = launch_small_rows<T>(q, st);
+    if (launches < 0) return -1;
+    grad_x = nullptr;
+    if (!grad_w && !grad_bias) return launches;
+  }
+  const bool products = grad_x || grad_w;
   Carver cv;
   // dz: grad_out itself when there is no activation and the products can read it
   Operand<T> dz(grad_out, a.rows, a.d_out, a.ldy, a.o.activation != 0, cv);
   Operand<T> x(a.x, a.rows, a.d_in, a.ldx, false, cv);
-  Operand<T> w(a.w, tw ? a.d_out : a.d_in, tw ? a.d_in : a.d_out, a.ldw, false, cv);
+  Carver none;  // an operand that no product reads takes no scratch
+  Operand<T> w(a.w, tw ? a.d_out : a.d_in, tw ? a.d_in : a.d_out, a.ldw, false, grad_x ? cv : none);
   ProductSpec s[2];
   LinProduct epi[2];
   memset(epi, 0, sizeof(epi));
@@ -1172,7 +1134,6 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
   if (!base) return -1;
   dz.bind(base); x.bind(base); w.bind(base);
   describe();
-  int launches = 0;
   if ((products && dz.copy) || grad_bias) {
     SlopeArgs q;
     q.grad_out = grad_out; q.pre = a.o.pre; q.dz = (products && dz.copy) ? const_cast<void*>(dz.s.p) : nullptr;
@@ -1252,7 +1213,8 @@ template <typename T> cudaError_t set_attributes_of() {
 }  // namespace
 
 cudaError_t linear_set_attributes() {
-  cudaError_t e = set_attributes_of<float>();
+  cudaError_t e = linear_small_set_attributes();
+  if (e == cudaSuccess) e = set_attributes_of<float>();
   if (e == cudaSuccess) e = set_attributes_of<__half>();
   if (e == cudaSuccess) e = set_attributes_of<__nv_bfloat16>();
   return e;

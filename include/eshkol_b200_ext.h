@@ -340,7 +340,7 @@ typedef struct EshkolB200LinearOpts {
 } EshkolB200LinearOpts;
 int eshkol_b200_linear_forward_device(const void* x, const void* w, void* y, uint64_t rows, uint64_t d_in,
                                       uint64_t d_out, const EshkolB200LinearOpts* opts);
-/* Its gradients: with dz = grad_out * activation'(pre), rounded to the storage type for the products,
+/* Its gradients: with dz = grad_out * activation'(pre), which 16-bit tensors round once for the products,
  *   grad_x = dz w^T,  grad_w = x^T dz (stored as w is),  grad_bias = column sums of the unrounded dz
  * grad_out [rows x d_out] has the pitch ldy, grad_x that of x, grad_w that of w; grad_bias [d_out] is f32.
  * Each result may be NULL, not all of them; x may be NULL without grad_w, w without grad_x.  opts->bias
