@@ -142,20 +142,45 @@ template <typename T, int kD> __device__ __forceinline__ Word<T> to_word(const D
   else return narrow_word(d);
 }
 
-// Sixteen bytes' worth of a row of n elements from element c: one word where `words` says that the row's
-// words are aligned and it lies whole in the row, else element by element, `otherwise` outside.
-template <typename T> __device__ __forceinline__ Word<T> read_word(const T* row, int c, int n, bool words, T otherwise) {
+// How the rows of a matrix may be accessed: in words of 16 bytes, (16-bit types) in pairs, one by one
+enum Access : int { kSingly = 0, kInPairs = 1, kInWords = 2 };
+
+// Sixteen bytes' worth of a row of n elements from element c, `otherwise` outside.  A word that does not lie
+// whole in the row goes element by element; pairs imply an even n.
+template <typename T> __device__ __forceinline__ Word<T> read_word(const T* row, int c, int n, int access, T otherwise) {
   constexpr int kV = kVec16<T>;
-  if (words && c + kV <= n) return *reinterpret_cast<const Word<T>*>(row + c);
+  if (access == kInWords && c + kV <= n) return *reinterpret_cast<const Word<T>*>(row + c);
   Word<T> p;
+  if (sizeof(T) == 2 && access == kInPairs) {
+#pragma unroll
+    for (int j = 0; j < kV; j += 2) {
+      Pack<T, 2> q;
+      q.v[0] = q.v[1] = otherwise;
+      if (c + j < n) q = *reinterpret_cast<const Pack<T, 2>*>(row + c + j);
+      p.v[j] = q.v[0];
+      p.v[j + 1] = q.v[1];
+    }
+    return p;
+  }
 #pragma unroll
   for (int j = 0; j < kV; ++j) p.v[j] = c + j < n ? row[c + j] : otherwise;
   return p;
 }
-template <typename T> __device__ __forceinline__ void write_word(T* row, int c, int n, bool words, const Word<T>& p) {
+template <typename T> __device__ __forceinline__ void write_word(T* row, int c, int n, int access, const Word<T>& p) {
   constexpr int kV = kVec16<T>;
-  if (words && c + kV <= n) {
+  if (access == kInWords && c + kV <= n) {
     *reinterpret_cast<Word<T>*>(row + c) = p;
+    return;
+  }
+  if (sizeof(T) == 2 && access == kInPairs) {
+#pragma unroll
+    for (int j = 0; j < kV; j += 2)
+      if (c + j < n) {
+        Pack<T, 2> q;
+        q.v[0] = p.v[j];
+        q.v[1] = p.v[j + 1];
+        *reinterpret_cast<Pack<T, 2>*>(row + c + j) = q;
+      }
     return;
   }
 #pragma unroll
@@ -222,16 +247,21 @@ template <int kLeft> __device__ __forceinline__ void wait_async() {
 }
 
 // How a row's words get from memory to the threads that work on them, some rows ahead: in registers, or
-// through shared memory in copies of words or of elements
+// through shared memory in copies of words or of elements (16-bit ones in pairs: an asynchronous copy moves
+// four bytes at least, so their rows must be even in length and lie on 4-byte boundaries)
 enum Ahead : int { kInRegisters = 0, kByWords = 1, kByElements = 2 };
+template <typename T> inline bool rows_by_elements(const void* p, long long ld, long long n) {
+  return sizeof(T) >= 4 || ((reinterpret_cast<uintptr_t>(p) & 3u) == 0 && ld % 2 == 0 && n % 2 == 0);
+}
 // starts the copy of the word at element c < n of a row into this thread's place
 template <typename T, int kHow> __device__ __forceinline__ void copy_word(Word<T>* place, const T* row, int c, int n) {
   if constexpr (kHow == kByWords) {
     copy_async16(place, row + c);
-  } else if constexpr (sizeof(T) >= 4) {
+  } else {
+    constexpr int kStep = sizeof(T) >= 4 ? 1 : 2;
 #pragma unroll
-    for (int j = 0; j < kVec16<T>; ++j)
-      if (c + j < n) copy_async_small<sizeof(T)>(&place->v[j], row + c + j);
+    for (int j = 0; j < kVec16<T>; j += kStep)
+      if (c + j < n) copy_async_small<sizeof(T) * kStep>(&place->v[j], row + c + j);
   }
 }
 // the copied word, `zero` behind the row
@@ -243,18 +273,22 @@ template <typename T, int kHow> __device__ __forceinline__ Word<T> take_word(con
   return p;
 }
 // read_word and write_word where kByWords promises that every word is aligned and whole, c < n
-template <typename T, int kHow> __device__ __forceinline__ Word<T> get_word(const T* row, int c, int n, bool words, T otherwise) {
+template <typename T, int kHow> __device__ __forceinline__ Word<T> get_word(const T* row, int c, int n, int access, T otherwise) {
   if constexpr (kHow == kByWords) return *reinterpret_cast<const Word<T>*>(row + c);
-  else return read_word(row, c, n, words, otherwise);
+  else return read_word(row, c, n, access, otherwise);
 }
-template <typename T, int kHow> __device__ __forceinline__ void put_word(T* row, int c, int n, bool words, const Word<T>& p) {
+template <typename T, int kHow> __device__ __forceinline__ void put_word(T* row, int c, int n, int access, const Word<T>& p) {
   if constexpr (kHow == kByWords) *reinterpret_cast<Word<T>*>(row + c) = p;
-  else write_word(row, c, n, words, p);
+  else write_word(row, c, n, access, p);
 }
 
 // A device pointer's alignment and a row pitch both a multiple of 16 bytes
 template <typename T> inline bool rows_on_16_bytes(const void* p, long long ld) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * static_cast<long long>(sizeof(T))) % 16 == 0;
+}
+
+template <typename T> inline int row_access(const void* p, long long ld, long long n) {
+  return rows_on_16_bytes<T>(p, ld) ? kInWords : sizeof(T) == 2 && rows_by_elements<T>(p, ld, n) ? kInPairs : kSingly;
 }
 
 // Makes the library's device current for one call and puts the caller's back.

@@ -34,7 +34,7 @@ struct NormArgs {
   void *y, *mean, *inv_std;
   long long rows, ldx, ldy;
   int n;
-  bool x_words, y_words, gamma_words, beta_words;  // rows on 16-byte boundaries
+  int x_access, y_access, gamma_access, beta_access;
   double epsilon;
 };
 
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 25
       stage = stage + 1 == kAhead ? 0 : stage + 1;
     } else {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) widen_word(read_word(in, (t + i * width) * kV, n, a.x_words, zero), d[i]);
+      for (int i = 0; i < kN; ++i) widen_word(read_word(in, (t + i * width) * kV, n, a.x_access, zero), d[i]);
       in += in_step;
     }
     D sum2[kD];
@@ -141,14 +141,14 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 25
       const int c = (t + i * width) * kV;
       if (c >= n) break;
       D g[kD], b[kD];
-      if (gamma) widen_word(get_word<T, kHow>(gamma, c, n, a.gamma_words, one), g);
-      if (beta) widen_word(get_word<T, kHow>(beta, c, n, a.beta_words, zero), b);
+      if (gamma) widen_word(get_word<T, kHow>(gamma, c, n, a.gamma_access, one), g);
+      if (beta) widen_word(get_word<T, kHow>(beta, c, n, a.beta_access, zero), b);
 #pragma unroll
       for (int j = 0; j < kD; ++j) {
         const D scale = gamma ? g[j] * both(r_std) : both(r_std), centred = d[i][j] + both(-off);
         d[i][j] = beta ? fma2(centred, scale, b[j]) : centred * scale;
       }
-      put_word<T, kHow>(out, c, n, a.y_words, to_word<T>(d[i]));
+      put_word<T, kHow>(out, c, n, a.y_access, to_word<T>(d[i]));
     }
     out += out_step;
   }
@@ -198,7 +198,7 @@ struct NormGradArgs {
   void *grad_in, *grad_gamma, *grad_beta, *partial;
   long long rows, ldg, ldx, ldi;
   int n;
-  bool g_words, x_words, i_words, gamma_words;
+  int g_access, x_access, i_access, gamma_access;
 };
 
 // A row belongs to a warp, to a block, or to the blocks of a cluster, each with a contiguous part of the
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, kWarp ? 3 : 512 / kThreads) layernor
   Word<T> w[kN];
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    w[i] = read_word(static_cast<const T*>(a.gamma), (t + i * width) * kV, a.gamma ? n : 0, a.gamma_words, Elem<T>::narrow(1));
+    w[i] = read_word(static_cast<const T*>(a.gamma), (t + i * width) * kV, a.gamma ? n : 0, a.gamma_access, Elem<T>::narrow(1));
 #pragma unroll
     for (int j = 0; j < kD; ++j) sum_g[i][j] = sum_gx[i][j] = both(A(0));
   }
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, kWarp ? 3 : 512 / kThreads) layernor
             copy_word<T, kHow>(place(stage, 1, i), grad_out, c, n);
           }
         } else {
-          px[i] = read_word(x, c, n, a.x_words, zero);
-          pg[i] = read_word(grad_out, c, n, a.g_words, zero);
+          px[i] = read_word(x, c, n, a.x_access, zero);
+          pg[i] = read_word(grad_out, c, n, a.g_access, zero);
         }
       }
       next_m[stage] = *mean;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, kWarp ? 3 : 512 / kThreads) layernor
         if (c >= n) break;
 #pragma unroll
         for (int j = 0; j < kD; ++j) u[i][j] = fma2(fma2(xhat[i][j], along, u[i][j]), both(rs), level);
-        put_word<T, kHow>(out, c, n, a.i_words, to_word<T>(u[i]));
+        put_word<T, kHow>(out, c, n, a.i_access, to_word<T>(u[i]));
       }
       out += i_step;
     }
@@ -495,10 +495,10 @@ template <typename T, int kHow> void launch_forward_many(const NormArgs& a, int 
 
 template <typename T> int launch_forward(NormArgs a, cudaStream_t st) {
   using A = typename Elem<T>::Acc;
-  a.x_words = rows_on_16_bytes<T>(a.x, a.ldx);
-  a.y_words = rows_on_16_bytes<T>(a.y, a.ldy);
-  a.gamma_words = rows_on_16_bytes<T>(a.gamma, 0);
-  a.beta_words = rows_on_16_bytes<T>(a.beta, 0);
+  a.x_access = row_access<T>(a.x, a.ldx, a.n);
+  a.y_access = row_access<T>(a.y, a.ldy, a.n);
+  a.gamma_access = row_access<T>(a.gamma, 0, a.n);
+  a.beta_access = row_access<T>(a.beta, 0, a.n);
   const int words = (a.n + kVec16<T> - 1) / kVec16<T>;
   const long long sms = lib_num_sms();
   if (words > 4096) {  // over four words for each of 1024 threads
@@ -511,10 +511,12 @@ template <typename T> int launch_forward(NormArgs a, cudaStream_t st) {
     else if (words <= 512) launch_forward_as<T, 1, false, 512, kInRegisters>(a, st);
     else if (words <= 1024) launch_forward_as<T, 1, false, 1024, kInRegisters>(a, st);
     else launch_forward_as<T, 4, false, 1024, kInRegisters>(a, st);
-  } else if (a.x_words && a.y_words && a.gamma_words && a.beta_words && a.n % kVec16<T> == 0) {
+  } else if (a.x_access == kInWords && a.y_access == kInWords && a.gamma_access == kInWords && a.beta_access == kInWords &&
+             a.n % kVec16<T> == 0) {
     launch_forward_many<T, kByWords>(a, words, st);
   } else {
-    launch_forward_many<T, sizeof(T) >= 4 ? kByElements : kInRegisters>(a, words, st);
+    if (rows_by_elements<T>(a.x, a.ldx, a.n)) launch_forward_many<T, kByElements>(a, words, st);
+    else launch_forward_many<T, kInRegisters>(a, words, st);
   }
   return 1;
 }
@@ -528,9 +530,9 @@ template <typename T> GradShape gradients_shape(const NormGradArgs& a) {
   const long long sms = lib_num_sms();
   const int words = (a.n + kV - 1) / kV;
   if (words <= 32 * kN) return {words <= 32 ? 1 : words <= 64 ? 2 : 4, 0, 1, grid_of((a.rows + 3) / 4, sms * 3)};
-  // a block takes up to 512 words; a wider row takes more blocks, at most eight
+  // a block takes up to 256 threads' words; a wider row takes more blocks, at most eight
   int threads = 64, parts = 1;
-  while (threads < 512 / kN && words > threads * kN) threads *= 2;
+  while (threads < 256 && words > threads * kN) threads *= 2;
   while (parts < 8 && words > threads * kN * parts) parts *= 2;
   if (words > threads * kN * parts) return {0, 0, 0, 0};
   return {kN, threads, parts, grid_of(a.rows, sms * (512 / threads) / parts)};
@@ -569,21 +571,24 @@ cudaError_t launch_gradients_shaped(const NormGradArgs& a, const GradShape& q, c
   }
   if (q.threads == 64) return launch_gradients_as<T, kN, false, 64, kHow>(a, q, st);
   if (q.threads == 128) return launch_gradients_as<T, kN, false, 128, kHow>(a, q, st);
-  return launch_gradients_as<T, kN, false, 512 / kN, kHow>(a, q, st);
+  return launch_gradients_as<T, kN, false, 256, kHow>(a, q, st);
 }
 template <typename T> cudaError_t launch_gradients_any(const NormGradArgs& a, const GradShape& q, cudaStream_t st) {
-  if (a.g_words && a.x_words && a.i_words && a.n % kVec16<T> == 0) return launch_gradients_shaped<T, kByWords>(a, q, st);
-  if constexpr (sizeof(T) >= 4) return launch_gradients_shaped<T, kByElements>(a, q, st);
+  if (a.g_access == kInWords && a.x_access == kInWords && a.i_access == kInWords && a.n % kVec16<T> == 0)
+    return launch_gradients_shaped<T, kByWords>(a, q, st);
+  if (rows_by_elements<T>(a.grad_out, a.ldg, a.n) && rows_by_elements<T>(a.x, a.ldx, a.n))
+    return launch_gradients_shaped<T, kByElements>(a, q, st);
+  if constexpr (sizeof(T) >= 4) return cudaErrorInvalidValue;  // any such row can be copied
   else return launch_gradients_shaped<T, kInRegisters>(a, q, st);
 }
 
 template <typename T>
 int launch_gradients(NormGradArgs a, OpScratch& scratch, cudaStream_t st) {
   using A = typename Elem<T>::Acc;
-  a.g_words = rows_on_16_bytes<T>(a.grad_out, a.ldg);
-  a.x_words = rows_on_16_bytes<T>(a.x, a.ldx);
-  a.i_words = rows_on_16_bytes<T>(a.grad_in, a.ldi);
-  a.gamma_words = rows_on_16_bytes<T>(a.gamma, 0);
+  a.g_access = row_access<T>(a.grad_out, a.ldg, a.n);
+  a.x_access = row_access<T>(a.x, a.ldx, a.n);
+  a.i_access = row_access<T>(a.grad_in, a.ldi, a.n);
+  a.gamma_access = row_access<T>(a.gamma, 0, a.n);
   const GradShape q = gradients_shape<T>(a);
   const bool weights = a.grad_gamma || a.grad_beta;
   const size_t row_of_sums = 2 * static_cast<size_t>(a.n) * sizeof(A);

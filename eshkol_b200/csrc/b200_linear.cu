@@ -244,16 +244,19 @@ __device__ __forceinline__ void finish_words(const LinEpilogue& e, const float* 
     }
   }
 }
-// Any other block goes through the warp's exchange tile, so that lanes next to each other write elements next
-// to each other.
-template <typename T>
-__device__ __forceinline__ void finish_singly(const LinEpilogue& e, float* tile, const float* bias, const uint32_t (&v)[32],
-                                              long long row0, int c0) {
-  const int lane = threadIdx.x & 31, c = c0 + lane;
-  const T* res_at = static_cast<const T*>(e.residual) + row0 * e.ld_res + c;
-  T* out_at = static_cast<T*>(e.out) + row0 * e.ldo + c;
-  T* pre_at = static_cast<T*>(e.pre) + row0 * e.ld_pre + c;
-  const float b[1] = {bias[lane]};
+// Any other block goes through the warp's exchange tile, so that lanes next to each other write elements, or
+// pairs of 16-bit ones where rows lie on 4-byte boundaries, next to each other.
+template <typename T, int kV>
+__device__ __forceinline__ void finish_through_tile(const LinEpilogue& e, float* tile, const float* bias, const uint32_t (&v)[32],
+                                                    long long row0, int c0) {
+  constexpr int kAcross = 32 / kV, kSteps = 16 / kV;  // lanes of a row, steps of kV rows in half a block
+  const int lane = threadIdx.x & 31, at = (lane % kAcross) * kV, c = c0 + at, r = lane / kAcross;
+  const T* res_at = static_cast<const T*>(e.residual) + (row0 + r) * e.ld_res + c;
+  T* out_at = static_cast<T*>(e.out) + (row0 + r) * e.ldo + c;
+  T* pre_at = static_cast<T*>(e.pre) + (row0 + r) * e.ld_pre + c;
+  float b[kV];
+#pragma unroll
+  for (int j = 0; j < kV; ++j) b[j] = bias[at + j];
 #pragma unroll 1
   for (int half = 0; half < 2; ++half) {
     __syncwarp();
@@ -265,21 +268,25 @@ __device__ __forceinline__ void finish_singly(const LinEpilogue& e, float* tile,
     __syncwarp();
     const long long left = e.M - row0 - 16 * half;
     const int rows = left < 16 ? static_cast<int>(left) : 16;
-    if (c < e.N) {
+    if (c < e.N) {  // pairs: N is even
 #pragma unroll 1
-      for (int r0 = 0; r0 < rows; r0 += 8) {  // eight rows on their way at a time
-        Pack<T, 1> res[8];
+      for (int s0 = 0; s0 < kSteps; s0 += 8) {  // eight steps on their way at a time
+        Pack<T, kV> res[8];
 #pragma unroll
         for (int s = 0; s < 8; ++s)
-          if (e.residual && r0 + s < rows) res[s].v[0] = res_at[(16 * half + r0 + s) * e.ld_res];
+          if (e.residual && r + (s0 + s) * kV < rows)
+            res[s] = *reinterpret_cast<const Pack<T, kV>*>(res_at + (16 * half + (s0 + s) * kV) * e.ld_res);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-          if (r0 + s >= rows) break;
-          const float acc[1] = {tile[(r0 + s) * kStagePitch + lane]};
-          Pack<T, 1> y, z;
-          finish_elements<T, 1>(e, acc, b, res[s], y, z);
-          out_at[(16 * half + r0 + s) * e.ldo] = y.v[0];
-          if (e.pre) pre_at[(16 * half + r0 + s) * e.ld_pre] = z.v[0];
+          const int row = r + (s0 + s) * kV;
+          if (row >= rows) break;
+          float acc[kV];
+#pragma unroll
+          for (int j = 0; j < kV; ++j) acc[j] = tile[row * kStagePitch + at + j];
+          Pack<T, kV> y, z;
+          finish_elements<T, kV>(e, acc, b, res[s], y, z);
+          *reinterpret_cast<Pack<T, kV>*>(out_at + (16 * half + (s0 + s) * kV) * e.ldo) = y;
+          if (e.pre) *reinterpret_cast<Pack<T, kV>*>(pre_at + (16 * half + (s0 + s) * kV) * e.ld_pre) = z;
         }
       }
     }
@@ -506,7 +513,8 @@ linear_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__ LinP
           if (cc + 1 < kBlocks) load_residual<T>(e, row, c0 + 32, res);  // the next block's
           finish_words<T>(e, bias + cc * 32, v, row, c0, now);
         } else {
-          finish_singly<T>(e, tile, bias + cc * 32, v, row0, c0);
+          if (sizeof(T) == 2 && e.pairs) finish_through_tile<T, sizeof(T) == 2 ? 2 : 1>(e, tile, bias + cc * 32, v, row0, c0);
+          else finish_through_tile<T, 1>(e, tile, bias + cc * 32, v, row0, c0);
         }
       };
       if constexpr (kPlanes == 1) {
@@ -750,8 +758,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) linear_slope_kern
       } else {
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-          g[w] = read_word(gr, c + w * kV, a.cols, false, zero);
-          if (a.act) z[w] = read_word(zr, c + w * kV, a.cols, false, zero);
+          g[w] = read_word(gr, c + w * kV, a.cols, kSingly, zero);
+          if (a.act) z[w] = read_word(zr, c + w * kV, a.cols, kSingly, zero);
         }
         gr += g_step;
         zr += z_step;
@@ -788,14 +796,20 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) linear_slope_kern
   for (int w = 0; w < 8; ++w) s += sm[w][threadIdx.x];
   if (col < a.cols) a.partial[static_cast<long long>(blockIdx.y) * a.cols + col] = s;
 }
-__global__ void __launch_bounds__(256) linear_bias_join_kernel(const float* __restrict__ partial, int parts, int cols,
-                                                               float* __restrict__ out) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+// the blocks' column sums added in a fixed order: 32 columns per block, 32 threads per column
+__global__ void __launch_bounds__(1024) linear_bias_join_kernel(const float* __restrict__ partial, int parts, int cols,
+                                                                float* __restrict__ out) {
+  __shared__ float sm[32][33];
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
   float s = 0.f;
+  if (c < cols) {
 #pragma unroll 8
-  for (int p = 0; p < parts; ++p) s += partial[static_cast<long long>(p) * cols + c];
-  out[c] = s;
+    for (int p = lane; p < parts; p += 32) s += partial[static_cast<long long>(p) * cols + c];
+  }
+  sm[lane][col] = s;
+  __syncthreads();
+  s = warp_sum(sm[col][lane]);  // a warp now holds the 32 shares of one column
+  if (col == 0 && blockIdx.x * 32 + lane < cols) out[blockIdx.x * 32 + lane] = s;
 }
 
 // ------------------------------------------------------------------ host side
@@ -946,6 +960,8 @@ int run_products(const ProductSpec* s, LinProduct* p, int n, const Plan& plan, u
     }
     q.e.words = rows_on_16_bytes<T>(q.e.out, q.e.ldo) && (!q.e.pre || rows_on_16_bytes<T>(q.e.pre, q.e.ld_pre)) &&
                 (!q.e.residual || rows_on_16_bytes<T>(q.e.residual, q.e.ld_res));
+    q.e.pairs = rows_by_elements<T>(q.e.out, q.e.ldo, q.e.N) && (!q.e.pre || rows_by_elements<T>(q.e.pre, q.e.ld_pre, q.e.N)) &&
+                (!q.e.residual || rows_by_elements<T>(q.e.residual, q.e.ld_res, q.e.N));
   }
   int workers = lib_num_sms();
   if (plan.pair) workers /= 2;
@@ -1142,13 +1158,14 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
     q.cols = static_cast<int>(a.d_out); q.act = a.o.activation;
     q.words = rows_on_16_bytes<T>(grad_out, a.ldy) && (!q.act || rows_on_16_bytes<T>(q.pre, a.ld_pre));
     const dim3 grid(static_cast<unsigned>(col_blocks), static_cast<unsigned>(row_blocks));
-    constexpr int kWhole = kByWords, kParts = sizeof(T) >= 4 ? kByElements : kInRegisters;
     constexpr size_t smem = static_cast<size_t>(kSlopeDepth) * 2 * (8 / kVec16<T>) * 256 * 16;
-    if (q.words && a.d_out % 8 == 0) linear_slope_kernel<T, kWhole><<<grid, 256, smem, st>>>(q);
-    else linear_slope_kernel<T, kParts><<<grid, 256, kParts == kInRegisters ? 0 : smem, st>>>(q);
+    if (q.words && a.d_out % 8 == 0) linear_slope_kernel<T, kByWords><<<grid, 256, smem, st>>>(q);
+    else if (rows_by_elements<T>(grad_out, a.ldy, a.d_out) && (!q.act || rows_by_elements<T>(q.pre, a.ld_pre, a.d_out)))
+      linear_slope_kernel<T, kByElements><<<grid, 256, smem, st>>>(q);
+    else linear_slope_kernel<T, kInRegisters><<<grid, 256, 0, st>>>(q);
     ++launches;
     if (grad_bias) {
-      linear_bias_join_kernel<<<static_cast<unsigned>(col_blocks), 256, 0, st>>>(
+      linear_bias_join_kernel<<<static_cast<unsigned>((a.d_out + 31) / 32), 1024, 0, st>>>(
           q.partial, static_cast<int>(row_blocks), q.cols, static_cast<float*>(grad_bias));
       ++launches;
     }
@@ -1195,10 +1212,8 @@ template <int BN, typename T, bool kPair> cudaError_t set_attribute() {
 template <typename T> cudaError_t set_attributes_of() {
   constexpr int kSlopeBytes = kSlopeDepth * 2 * (8 / kVec16<T>) * 256 * 16;
   cudaError_t e = cudaFuncSetAttribute(linear_slope_kernel<T, kByWords>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlopeBytes);
-  if constexpr (sizeof(T) >= 4) {
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(linear_slope_kernel<T, kByElements>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlopeBytes);
-  }
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(linear_slope_kernel<T, kByElements>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlopeBytes);
   if (e == cudaSuccess) e = set_attribute<128, T, false>();
   if (e == cudaSuccess) e = set_attribute<64, T, false>();
   if constexpr (Plane<T>::kCount == 1) {

@@ -11,6 +11,7 @@ struct LinEpilogue {
   long long ldo, ld_res, ld_pre;
   int M, N, act;
   int words;              // 1: out, pre and residual rows lie on 16-byte boundaries
+  int pairs;              // 1: N is even and those rows lie on 4-byte boundaries (16-bit types)
 };
 
 // ------------------------------------------------------------------ activations
