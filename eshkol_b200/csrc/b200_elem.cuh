@@ -325,5 +325,6 @@ class OpScratch {
   cudaStream_t st_ = nullptr;
 };
 void op_scratch_shutdown();
+size_t op_scratch_bytes();
 
 }  // namespace b200

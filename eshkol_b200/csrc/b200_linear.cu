@@ -14,6 +14,9 @@
 // but for the last rounding, relative 2^-27), and six of the nine products of the parts make the result;
 // the three left out are below 2^-26 of the terms.
 //
+// Bound by the tensor pipe (active 94 % of the time on pairs of SMs): 8192 x 16384 x 4096 bf16 takes 725 us in
+// a burst, 1517 TFLOP/s, and 850 under the power cap; all gradients at 4096 x 4096 x 16384 755 us in a burst.
+//
 // A few rows: b200_linear_small.cu.  Few output tiles and a long reduction: the reduction is split over blocks, their f32 sums go to scratch
 // and a second kernel adds them in order and applies the epilogue.
 #include <math.h>
@@ -47,8 +50,8 @@ template <> struct Plane<float> { using type = __nv_bfloat16; static constexpr i
 // f32: k-blocks of 32, the three planes of both operands in a stage, so that their six products cost the
 // loads of three; two accumulators, the product of the leading parts in one and the rest, 2^-8 of it, in
 // the other, handed over every kDrain k-blocks and added up in registers: the tensor core truncates its
-// sums, and 16 truncations in a row are as many as the result's accuracy bears (measured: 126 in a row left
-// 2e-6 of the norm, 16 leave 4e-7).
+// sums, and 16 truncations in a row are as many as the result's accuracy bears (measured at K = 2001: 126 in
+// a row left 2e-6 of the norm, 16 leave 2.3e-7, a plain f32 product 7.7e-7).
 template <int BN, typename T, bool kPair> struct LinShape {
   static constexpr int kPlanes = Plane<T>::kCount;
   static constexpr int kBK = kPlanes == 3 ? 32 : 64;       // elements per k-block: 64- or 128-byte swizzle rows

@@ -59,6 +59,8 @@ int OpScratch::release() {
   return 0;
 }
 
+size_t op_scratch_bytes() { return g_bytes; }
+
 void op_scratch_shutdown() {
   if (g_block) cudaFree(g_block);
   g_block = nullptr;

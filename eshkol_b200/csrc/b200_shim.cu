@@ -1844,7 +1844,7 @@ void eshkol_b200_debug_fail_allocation(int nth) { g_dbg_fail_alloc = nth > 0 ? n
 void eshkol_b200_debug_withhold_arrival(int on) { g_dbg_withhold = on ? 1 : 0; }
 
 uint64_t eshkol_b200_launch_count(void) { return g.launches; }
-uint64_t eshkol_b200_workspace_bytes(void) { return g.ws_bytes + g.aux_bytes + g.bside_bytes; }
+uint64_t eshkol_b200_workspace_bytes(void) { return g.ws_bytes + g.aux_bytes + g.bside_bytes + op_scratch_bytes(); }
 
 int eshkol_b200_debug_fetch(int what, int index, void* host_dst, uint64_t capacity_bytes,
                             uint64_t info[6]) {
