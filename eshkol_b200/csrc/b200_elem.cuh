@@ -246,6 +246,31 @@ template <int kLeft> __device__ __forceinline__ void wait_async() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
+// Launches of one operator that follow one another (launch_after): the next kernel's blocks may come to the
+// SMs as soon as all blocks of the one before have called let_next_start, and wait in after_previous, their
+// first instruction, until that kernel is complete and its writes are visible.  That hides the start of the
+// launch, 1 to 2 us.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+inline cudaLaunchAttribute after_attribute() {
+  cudaLaunchAttribute a;
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+template <typename... Params, typename... Args>
+inline cudaError_t launch_after(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t shared, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = st;
+  cudaLaunchAttribute attr = after_attribute();
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // How a row's words get from memory to the threads that work on them, some rows ahead: in registers, or
 // through shared memory in copies of words or of elements (16-bit ones in pairs: an asynchronous copy moves
 // four bytes at least, so their rows must be even in length and lie on 4-byte boundaries)

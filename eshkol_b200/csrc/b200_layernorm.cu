@@ -9,7 +9,7 @@
 // one write, so the statistics are the two-pass ones (the mean first, then the deviations, with the
 // deviations' own sum as a correction) at the traffic of one pass.  What bounds the kernels is instruction
 // issue and the latency of a row's reductions: 8192 x 4096 bf16 takes 39 us (3.4 TB/s, 0.53 of the measured
-// copy rate), its gradients at 16384 x 4096 88 us (4.6 TB/s, 0.70).  Sums, statistics and the weights'
+// copy rate), its gradients at 16384 x 4096 87 us (4.6 TB/s, 0.71).  Sums, statistics and the weights'
 // gradients are f32 (f64 for f64 tensors); a result is rounded to the storage type once.  Sums are combined in
 // a fixed order: results do not depend on timing.
 #include <math.h>
@@ -46,13 +46,13 @@ struct NormArgs {
 // about ten (packed f32 arithmetic), so a thread gets four words where rows are many.  The next kAhead
 // rows are on their way in shared memory: every thread copies the words that it will read itself.  Measured at
 // 8192 x 4096 bf16: 128 threads with four words 39 us, 64 with eight 46, a warp with sixteen 53.
-template <int kHow> constexpr int kNormAhead = kHow == kInRegisters ? 1 : 4;
+template <int kThreads, int kHow> constexpr int kNormAhead = kHow == kInRegisters ? 1 : kThreads == 1024 ? 2 : 4;
 
 template <typename T, int kN, bool kWarp, int kThreads, int kHow>
 __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 256 ? 3 : 1) layernorm_kernel(const NormArgs a) {  // x and y may be the same
   using A = typename Elem<T>::Acc;
   using D = Duo<A>;
-  constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kNormAhead<kHow>;
+  constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kNormAhead<kThreads, kHow>;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ A sm1[32], sm2[64];
   constexpr int width = kWarp ? 32 : kThreads, warps = kWarp ? 1 : kThreads / 32, per_block = kWarp ? kThreads / 32 : 1;
@@ -218,6 +218,7 @@ template <typename T, int kN, bool kWarp, int kThreads, int kHow>
 __global__ void __launch_bounds__(kThreads, kWarp ? 3 : 512 / kThreads) layernorm_gradients_kernel(const NormGradArgs a) {
   using A = typename Elem<T>::Acc;
   using D = Duo<A>;
+  let_next_start();
   constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kRowsAhead<kN, kHow>;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ A sm[2][64];
@@ -446,6 +447,7 @@ template <typename A>
 __global__ void __launch_bounds__(1024) layernorm_join_kernel(const A* __restrict__ partial, int groups, int n,
                                                               A* __restrict__ grad_gamma, A* __restrict__ grad_beta) {
   __shared__ A sm[32][33];
+  after_previous();
   const int col = threadIdx.x & 31, lane = threadIdx.x >> 5;
   const long long c = static_cast<long long>(blockIdx.x) * 32 + col, width = 2LL * n;
   A s = 0;
@@ -475,7 +477,7 @@ template <typename F> bool allow_shared(F kernel, size_t bytes) {
 
 template <typename T, int kN, bool kWarp, int kThreads, int kHow>
 void launch_forward_as(const NormArgs& a, cudaStream_t st) {
-  constexpr size_t smem = kHow == kInRegisters ? 0 : static_cast<size_t>(kNormAhead<kHow>) * kN * kThreads * 16;
+  constexpr size_t smem = kHow == kInRegisters ? 0 : static_cast<size_t>(kNormAhead<kThreads, kHow>) * kN * kThreads * 16;
   const auto kernel = layernorm_kernel<T, kN, kWarp, kThreads, kHow>;
   if (!allow_shared(kernel, smem)) return;  // the error is read after the launch
   // blocks that an SM holds, by registers (the launch bounds) and by shared memory
@@ -493,7 +495,7 @@ template <typename T, int kHow> void launch_forward_many(const NormArgs& a, int 
   else if (words <= 512) launch_forward_as<T, 4, false, 128, kHow>(a, st);
   else if (words <= 1024) launch_forward_as<T, 4, false, 256, kHow>(a, st);
   else if (words <= 2048) launch_forward_as<T, 4, false, 512, kHow>(a, st);
-  else launch_forward_as<T, 4, false, 1024, kInRegisters>(a, st);
+  else launch_forward_as<T, 4, false, 1024, kHow>(a, st);
 }
 
 template <typename T> int launch_forward(NormArgs a, cudaStream_t st) {
@@ -627,8 +629,14 @@ int launch_gradients(NormGradArgs a, OpScratch& scratch, cudaStream_t st) {
     launches = 2;
   }
   if (weights) {
-    layernorm_join_kernel<A><<<static_cast<unsigned>((2LL * a.n + 31) / 32), 1024, 0, st>>>(
-        static_cast<const A*>(a.partial), groups, a.n, static_cast<A*>(a.grad_gamma), static_cast<A*>(a.grad_beta));
+    const cudaError_t e = launch_after(layernorm_join_kernel<A>, static_cast<unsigned>((2LL * a.n + 31) / 32), 1024, 0, st,
+                                       static_cast<const A*>(a.partial), groups, a.n, static_cast<A*>(a.grad_gamma),
+                                       static_cast<A*>(a.grad_beta));
+    if (e != cudaSuccess) {
+      fprintf(stderr, "[eshkol-b200] layer norm launch failed: %s\n", cudaGetErrorString(e));
+      cudaGetLastError();
+      return -1;
+    }
     ++launches;
   }
   return launches;

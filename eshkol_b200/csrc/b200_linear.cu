@@ -340,6 +340,8 @@ linear_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__ LinP
   if (kPair) pair_sync();  // the other SM's barriers exist before anything is signalled on them
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  after_previous();  // operands may come from the kernel before
+  let_next_start();
   LinSchedule schedule(prm, worker);
   LinWork it;
 
@@ -584,6 +586,8 @@ linear_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__ LinP
 // the partial sums of a split reduction, added in order, and the epilogue
 template <typename T>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinProduct q) {
+  after_previous();
+  let_next_start();
   const LinEpilogue e = q.e;
   const long long words = q.ldp / 4, total = e.M * words, slab = e.M * q.ldp;
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total;
@@ -683,6 +687,8 @@ struct PackJobs {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) linear_pack_kernel(const __grid_constant__ PackJobs jobs) {
+  after_previous();
+  let_next_start();
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < jobs.total;
        i += static_cast<long long>(gridDim.x) * 256) {
     const PackJob& q = jobs.j[(jobs.n > 1 && i >= jobs.j[1].first) ? 1 : 0];
@@ -711,6 +717,7 @@ template <typename T, int kHow>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) linear_slope_kernel(const __grid_constant__ SlopeArgs a) {
   constexpr bool kExact = sizeof(T) == 4;
   constexpr int kV = kVec16<T>, kD = kDuos<T>, kWords = 8 / kV;
+  let_next_start();
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ float sm[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -803,6 +810,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) linear_slope_kern
 __global__ void __launch_bounds__(1024) linear_bias_join_kernel(const float* __restrict__ partial, int parts, int cols,
                                                                 float* __restrict__ out) {
   __shared__ float sm[32][33];
+  after_previous();
+  let_next_start();
   const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
   float s = 0.f;
   if (c < cols) {
@@ -834,7 +843,7 @@ struct ProductSpec {
 };
 
 template <int BN, typename T, bool kPair>
-int launch_products(const ProductSpec* s, LinProduct* p, int n, LinParams& prm, cudaStream_t st) {
+int launch_products(const ProductSpec* s, LinProduct* p, int n, LinParams& prm, bool follows, cudaStream_t st) {
   using Shape = LinShape<BN, T, kPair>;
   LinMaps maps;
   for (int i = 0; i < n; ++i) {
@@ -853,12 +862,13 @@ int launch_products(const ProductSpec* s, LinProduct* p, int n, LinParams& prm, 
   cfg.blockDim = dim3(kLinThreads);
   cfg.dynamicSmemBytes = Shape::kSmem;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = kPair ? 2 : 1;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kPair ? 2 : 1;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1] = after_attribute();
+  cfg.attrs = attr;
+  cfg.numAttrs = follows ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_kernel<BN, T, kPair>, maps, prm);
   if (e != cudaSuccess) {
     fprintf(stderr, "[eshkol-b200] linear layer launch failed: %s\n", cudaGetErrorString(e));
@@ -866,6 +876,11 @@ int launch_products(const ProductSpec* s, LinProduct* p, int n, LinParams& prm, 
     return -1;
   }
   return 1;
+}
+
+int failed() {
+  fprintf(stderr, "[eshkol-b200] linear layer launch failed: %s\n", cudaGetErrorString(cudaGetLastError()));
+  return -1;
 }
 
 struct Plan {
@@ -933,9 +948,11 @@ template <typename T> Plan plan_products(const ProductSpec* s, int n) {
 }
 
 // Multiplies one or two independent products in one launch, and joins those whose reduction was split.
-// p[i].e carries the epilogue of product i; scratch_at: room for the partial sums (plan.partial_bytes).
+// p[i].e carries the epilogue of product i; scratch_at: room for the partial sums (plan.partial_bytes); follows:
+// a kernel of this call went before.
 template <typename T>
-int run_products(const ProductSpec* s, LinProduct* p, int n, const Plan& plan, uint8_t* scratch_at, cudaStream_t st) {
+int run_products(const ProductSpec* s, LinProduct* p, int n, const Plan& plan, uint8_t* scratch_at, bool follows,
+                 cudaStream_t st) {
   constexpr int kBK = Plane<T>::kCount == 3 ? 32 : 64;
   LinParams prm;
   memset(&prm, 0, sizeof(prm));
@@ -983,21 +1000,22 @@ int run_products(const ProductSpec* s, LinProduct* p, int n, const Plan& plan, u
   prm.withhold = lib_take_withhold();
   int launches = -1;
   if constexpr (Plane<T>::kCount == 3) {
-    launches = plan.pair       ? launch_products<128, T, true>(s, p, n, prm, st)
-               : plan.bn == 128 ? launch_products<128, T, false>(s, p, n, prm, st)
-                                : launch_products<64, T, false>(s, p, n, prm, st);
+    launches = plan.pair       ? launch_products<128, T, true>(s, p, n, prm, follows, st)
+               : plan.bn == 128 ? launch_products<128, T, false>(s, p, n, prm, follows, st)
+                                : launch_products<64, T, false>(s, p, n, prm, follows, st);
   } else {
-    launches = plan.pair        ? launch_products<256, T, true>(s, p, n, prm, st)
-               : plan.bn == 256 ? launch_products<256, T, false>(s, p, n, prm, st)
-               : plan.bn == 128 ? launch_products<128, T, false>(s, p, n, prm, st)
-                                : launch_products<64, T, false>(s, p, n, prm, st);
+    launches = plan.pair        ? launch_products<256, T, true>(s, p, n, prm, follows, st)
+               : plan.bn == 256 ? launch_products<256, T, false>(s, p, n, prm, follows, st)
+               : plan.bn == 128 ? launch_products<128, T, false>(s, p, n, prm, follows, st)
+                                : launch_products<64, T, false>(s, p, n, prm, follows, st);
   }
   if (launches < 0) return -1;
   for (int i = 0; i < n; ++i) {
     if (p[i].splits == 1) continue;
     const long long words = p[i].ldp / 4 * p[i].e.M, cap = static_cast<long long>(lib_num_sms()) * 8;
     const long long blocks = (words + 255) / 256;
-    linear_join_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, st>>>(p[i]);
+    if (launch_after(linear_join_kernel<T>, static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, st, p[i]) != cudaSuccess)
+      return failed();
     ++launches;
   }
   return launches;
@@ -1051,10 +1069,12 @@ template <typename T> void add_pack(PackJobs& jobs, const void* src, long long l
   jobs.total += j.rows * (j.ldd / 8);
   ++jobs.n;
 }
-template <typename T> int launch_pack(const PackJobs& jobs, cudaStream_t st) {
+template <typename T> int launch_pack(const PackJobs& jobs, bool follows, cudaStream_t st) {
   if (jobs.n == 0) return 0;
   const long long blocks = (jobs.total + 255) / 256, cap = static_cast<long long>(lib_num_sms()) * 16;
-  linear_pack_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, st>>>(jobs);
+  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+  if (!follows) linear_pack_kernel<T><<<grid, 256, 0, st>>>(jobs);
+  else if (launch_after(linear_pack_kernel<T>, grid, 256, 0, st, jobs) != cudaSuccess) return failed();
   return 1;
 }
 
@@ -1092,8 +1112,8 @@ template <typename T> int linear_forward(const LinearArgs& a, void* y, OpScratch
   PackJobs jobs = {};
   add_pack<T>(jobs, a.x, a.ldx, x);
   add_pack<T>(jobs, a.w, a.ldw, w);
-  const int packs = launch_pack<T>(jobs, st);
-  const int n = run_products<T>(&s, &epi, 1, plan, base + parts, st);
+  const int packs = launch_pack<T>(jobs, false, st);
+  const int n = run_products<T>(&s, &epi, 1, plan, base + parts, packs > 0, st);
   return n < 0 ? -1 : packs + n;
 }
 
@@ -1168,8 +1188,10 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
     else linear_slope_kernel<T, kInRegisters><<<grid, 256, 0, st>>>(q);
     ++launches;
     if (grad_bias) {
-      linear_bias_join_kernel<<<static_cast<unsigned>((a.d_out + 31) / 32), 1024, 0, st>>>(
-          q.partial, static_cast<int>(row_blocks), q.cols, static_cast<float*>(grad_bias));
+      if (launch_after(linear_bias_join_kernel, static_cast<unsigned>((a.d_out + 31) / 32), 1024, 0, st,
+                       static_cast<const float*>(q.partial), static_cast<int>(row_blocks), q.cols,
+                       static_cast<float*>(grad_bias)) != cudaSuccess)
+        return failed();
       ++launches;
     }
   }
@@ -1177,9 +1199,11 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
   PackJobs jobs = {};
   if (grad_w) add_pack<T>(jobs, a.x, a.ldx, x);
   if (grad_x) add_pack<T>(jobs, a.w, a.ldw, w);
-  launches += launch_pack<T>(jobs, st);
-  const int m = run_products<T>(s, epi, n, plan, base + parts, st);
-  return m < 0 ? -1 : launches + m;
+  const bool sloped = (products && dz.copy) || grad_bias;
+  const int packs = launch_pack<T>(jobs, sloped, st);
+  if (packs < 0) return -1;
+  const int m = run_products<T>(s, epi, n, plan, base + parts, sloped || packs > 0, st);
+  return m < 0 ? -1 : launches + packs + m;
 }
 
 bool pitch_ok(int64_t ld, uint64_t n) { return ld == 0 || (ld >= static_cast<int64_t>(n) && ld <= (1ll << 36)); }
