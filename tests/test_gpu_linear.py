@@ -18,7 +18,8 @@ pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1, 1, 0, 0), (3, 5, 7, 0, 0), (1, 64, 64, 0, 0), (1, 4096, 304, 0, 0), (17, 1001, 999, 0, 0),
           (128, 256, 512, 0, 0), (130, 300, 520, 8, 8), (257, 1000, 136, 5, 3), (300, 2048, 2048, 0, 0),
-          (64, 8192, 192, 0, 0), (700, 96, 40, 16, 8), (1000, 72, 1100, 1, 1)]
+          (64, 8192, 192, 0, 0), (700, 96, 40, 16, 8), (1000, 72, 1100, 1, 1), (2, 640, 384, 0, 0), (4, 1000, 520, 0, 0),
+          (8, 1030, 514, 1, 1), (12, 600, 250, 0, 0), (40, 90, 254, 2, 2), (520, 520, 1040, 0, 0)]
 
 
 def steps(k, dtype):
@@ -148,6 +149,25 @@ def test_special_values_stay_in_their_rows(gpu_lib):
     assert np.isnan(got[7]).all() and not np.isfinite(got[9]).any()
     keep = [r for r in range(50) if r not in (7, 9)]
     assert np.isfinite(got[keep]).all() and (got[50:] == 5.0).all()
+
+
+def test_products_of_two_rounds_and_more(gpu_lib):
+    """More tiles than SMs in both products of the gradients, unevenly: every tile is written once."""
+    import torch
+    t, tag, wt, u, half = kinds("bf16")
+    rows, k, n = 2100, 2300, 4200
+    x, w, g = (torch.randint(-1, 2, s, device="cuda").to(t) for s in ((rows, k), (k, n), (rows, n)))
+    x[:, 60:] = 0  # keeps the sums within the integers of bf16
+    g[:, 60:] = 0
+    g[60:] = 0
+    gx, gw, y = room((rows, k), t), room((k, n), t), room((rows, n), t)
+    eb.linear_device(x.data_ptr(), w.data_ptr(), y.data_ptr(), rows, k, n, eb.make_linear_opts(tag))
+    eb.linear_gradients_device(g.data_ptr(), x.data_ptr(), w.data_ptr(), gx.data_ptr(), gw.data_ptr(), 0, rows, k, n, eb.make_linear_opts(tag))
+    done()
+    f = [v.to(torch.float64) for v in (x, w, g)]
+    assert torch.equal(y.to(torch.float64), f[0] @ f[1])
+    assert torch.equal(gx.to(torch.float64), f[2] @ f[1].T)
+    assert torch.equal(gw.to(torch.float64), f[0].T @ f[2])
 
 
 def test_gelu_far_out(gpu_lib):

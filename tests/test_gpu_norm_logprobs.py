@@ -74,7 +74,8 @@ def untouched(view, offset):
 
 
 SHAPES = [(1, 1, 0, 0), (1, 4096, 0, 0), (3, 7, 0, 0), (1000, 40, 8, 8), (37, 1000, 0, 0), (130, 1001, 6, 1),
-          (2000, 256, 0, 0), (5, 5000, 3, 2), (700, 2048, 0, 0), (3, 20000, 0, 0), (150, 9001, 0, 0), (2, 70000, 1, 1)]
+          (2000, 256, 0, 0), (5, 5000, 3, 2), (700, 2048, 0, 0), (3, 20000, 0, 0), (150, 9001, 0, 0), (2, 70000, 1, 1),
+          (900, 810, 0, 0), (70, 5678, 2, 2), (640, 16390, 0, 0), (1300, 130, 1, 0)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -164,10 +165,13 @@ def logits(seed, rows, vocab, coarse=False):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocab,pad,offset", VOCABS)
-@pytest.mark.parametrize("how", ["plain", "ties", "masked"])
+@pytest.mark.parametrize("how", ["plain", "ties", "masked", "equal"])
 def test_token_logprobs(gpu_lib, dtype, rows, vocab, pad, offset, how):
     t, tag, wt, u, half = kinds(dtype)
     v = logits(61, rows, vocab, coarse=how == "ties")
+    if how == "equal":  # more ties than there is room for candidates: the lowest indices win
+        v[:] = 0.5
+        v[0, vocab // 3:] = 0.25
     if how == "masked":
         v[inputs.uniform(62, (rows, vocab)) < 0.2] = -np.inf
         v[0, :] = -np.inf
