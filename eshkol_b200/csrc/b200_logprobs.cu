@@ -137,6 +137,7 @@ template <typename A> constexpr A kFar = A(-1e30);  // exp of it is zero, a prod
 template <typename A> __device__ __forceinline__ A lowest();
 template <> __device__ __forceinline__ float lowest<float>() { return -3.402823466e38f; }
 template <> __device__ __forceinline__ double lowest<double>() { return -1.7976931348623157e308; }
+constexpr float kNear = 64.f;  // references up to here may be multiplied by log2 e before the subtraction
 template <typename A> constexpr A kSlack = A(4);  // how far a value may pass the reference before it moves
 
 // s and t relative to the finite reference m
@@ -278,20 +279,30 @@ template <typename T> struct Running {
     // exp(x - m) may grow to exp(4): as exact as below one, and the reference seldom moves
     if (top > m + kSlack<A>) move(top);
     if constexpr (sizeof(T) == 2) {
-      // (x - m) log2 e in one instruction: its rounding, 2^-25 of m log2 e, shifts all of the thread's
-      // exponents alike and comes to about half a step of the f32 result lse; t in units of log 2
-      const Duo<A> minus = both(-m * kLog2e), scale = both(kLog2e);
+      // (x - m) log2 e; t in units of log 2
+      const Duo<A> scale = both(kLog2e);
       Duo<A> t2 = both(A(0));
+      const auto sums = [&](auto exponent) {
 #pragma unroll
-      for (int u = 0; u < kWords; ++u) {
-        Duo<A> x[kDuos<T>];
-        widen_word(without_infinity(p[u]), x);
+        for (int u = 0; u < kWords; ++u) {
+          Duo<A> x[kDuos<T>];
+          widen_word(without_infinity(p[u]), x);
 #pragma unroll
-        for (int j = 0; j < kDuos<T>; ++j) {
-          const Duo<A> d = fma2(x[j], scale, minus), e = exp2_both(d);
-          s = s + e;
-          t2 = fma2(e, d, t2);
+          for (int j = 0; j < kDuos<T>; ++j) {
+            const Duo<A> d = exponent(x[j]), e = exp2_both(d);
+            s = s + e;
+            t2 = fma2(e, d, t2);
+          }
         }
+      };
+      if (fabsf(m) <= kNear) {
+        // one instruction: the roundings of log2 e and of m log2 e, 2^-26 + 2^-25 of m, shift all of the
+        // thread's exponents alike, by less than 3e-6
+        const Duo<A> minus = both(-m * kLog2e);
+        sums([&](Duo<A> x) { return fma2(x, scale, minus); });
+      } else {
+        const Duo<A> minus = both(-m);
+        sums([&](Duo<A> x) { return (x + minus) * scale; });
       }
       t = fma2(t2, both(kLn2), t);
     } else {

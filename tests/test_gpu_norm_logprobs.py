@@ -211,6 +211,30 @@ def test_token_logprobs(gpu_lib, dtype, rows, vocab, pad, offset, how):
     close(ent, w_ent, 2 * s * (2.0 + np.log(vocab)) * np.ones(rows))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [700, 5000, 40000])
+def test_token_logprobs_far_from_zero(gpu_lib, dtype, vocab):
+    """Rows around a large level, as additive masks leave them: differences from the largest logit decide."""
+    import torch
+    t, tag, wt, u, half = kinds(dtype)
+    levels = [0.0, 60.0, -70.0, 300.0, -5000.0, 60000.0] + ([] if dtype == "f16" else [1e6, -1e9, 1e12, -1e30, 1e35])
+    rows = len(levels)
+    x = laid(np.array(levels)[:, None] + inputs.normal(63, (rows, vocab)), t)
+    tokens = torch.arange(rows, device="cuda") * 7
+    lp, ent, lse = room((rows,), wt), room((rows,), wt), room((rows,), wt)
+    eb.token_logprobs_device(x.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), 0, 0, rows,
+                             vocab, 0, tag)
+    done()
+    xs = wide64(x)
+    y = xs - xs.max(axis=1, keepdims=True)  # the same probabilities, and logprob without cancellation
+    w_lp, w_ent, w_norm, _, _ = ref.token_logprobs(y, tokens.cpu().numpy(), 1)
+    s = 300 * u  # as above
+    w_lse = xs.max(axis=1) + w_norm
+    assert np.all(np.abs(wide64(lse) - w_lse) <= s + 2 * u * np.abs(w_lse))
+    assert np.all(np.abs(wide64(lp) - w_lp) <= s + 4 * u * (np.abs(w_lp) + w_norm))
+    assert np.all(np.abs(wide64(ent) - w_ent) <= 2 * s * (2.0 + np.log(vocab)))
+
+
 def test_token_logprobs_outputs_are_optional(gpu_lib):
     import torch
     t, tag, wt, u, half = kinds("bf16")
