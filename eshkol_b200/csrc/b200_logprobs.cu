@@ -15,8 +15,8 @@
 // larger logit first, equal logits by index, kept exactly by comparing (logit, index) as one key; a
 // candidate's rank is the number of better candidates.
 //
-// 4096 x 50257 bf16 with 8 alternatives takes 101 us (4.1 TB/s, 0.62 of the measured copy rate; without them
-// 86), bound by instruction issue and the exponential unit, one exponential an element: 46 us by itself.  The
+// 4096 x 50257 bf16 with 8 alternatives takes 108 us (3.8 TB/s, 0.58 of the measured copy rate; without them
+// 88), bound by instruction issue and the exponential unit, one exponential an element: 46 us by itself.  The
 // gradient takes 134 us (6.1 TB/s, 0.94).
 //
 // Entries of minus infinity have probability zero and add nothing.  A row of nothing else has lse minus
