@@ -133,7 +133,9 @@ __device__ __forceinline__ float floor_at(float v, float bound) {
   return r;
 }
 __device__ __forceinline__ double floor_at(double v, double bound) { return v < bound ? bound : v; }
-template <typename A> constexpr A kFar = A(-1e30);  // exp of it is zero, a product with it finite
+// Where differences end: exp of it is zero in f32 and f64, and so is a sum's or a gradient's part with it, while
+// its product with a factor as large as 10^35 (f32) is still finite: zero times infinity would be NaN.
+template <typename A> constexpr A kFar = A(-1e3);
 template <typename A> __device__ __forceinline__ A lowest();
 template <> __device__ __forceinline__ float lowest<float>() { return -3.402823466e38f; }
 template <> __device__ __forceinline__ double lowest<double>() { return -1.7976931348623157e308; }
