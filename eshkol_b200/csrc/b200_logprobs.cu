@@ -20,7 +20,8 @@
 // gradient takes 134 us (6.1 TB/s, 0.94).
 //
 // Entries of minus infinity have probability zero and add nothing.  A row of nothing else has lse minus
-// infinity, entropy zero and a zero gradient.  NaN or plus infinity makes the row's outputs NaN.
+// infinity, entropy zero and, for a gradient, g at the token and zeros.  NaN or plus infinity makes the row's
+// outputs NaN.
 #include <math.h>
 #include <stdio.h>
 

@@ -365,7 +365,8 @@ int eshkol_b200_token_logprobs_device(const void* logits, const int64_t* tokens,
  *   grad_logits[j] = grad_logprob * ([j = token] - p[j]) - grad_entropy * p[j] * (log p[j] + entropy)
  * grad_logprob or grad_entropy (stat type, [rows]) may be NULL, not both; entropy may be NULL without
  * grad_entropy, tokens without grad_logprob.  Positions without a token get no gradient from
- * grad_logprob; a token >= vocab makes its row NaN; a row without unmasked entries gets zeros.
+ * grad_logprob; a token >= vocab makes its row NaN.
+ * In a row without unmasked entries every p is 0: it gets grad_logprob at its token and zeros elsewhere.
  * p is exp(logits - lse) with lse as given: around a level of L it carries the rounding of lse, 2^-24 L in f32.
  * grad_logits may be logits with the same pitch. */
 int eshkol_b200_token_logprobs_gradient_device(const void* logits, const int64_t* tokens, const void* lse,

@@ -46,3 +46,27 @@ def test_a_large_gradient_of_the_entropy_meets_masked_entries(gpu_lib, dtype, vo
     mag = p * (np.abs(gs)[:, None] + np.abs(hs)[:, None] * (np.abs(lp) + np.abs(es)[:, None]))
     tol = half * np.abs(want) + (16 + 8 * np.abs(lp)) * u * mag + 2 * u * np.abs(gs)[:, None] + (2.0 ** -25 if dtype == "f16" else 0.0)
     assert np.all(np.abs(got - want) <= tol + (0 if dtype == "f64" else 2.0 ** -126 * 200 * np.abs(hs)[:, None]))
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 7, 900, 20001])
+def test_a_row_without_unmasked_entries(gpu_lib, dtype, vocab):
+    """All its probabilities are zero: what is left of the formula is grad_logprob at the token, and zeros."""
+    t, tag, wt, u, half = kinds(dtype)
+    x = laid(np.full((4, vocab), -np.inf), t)
+    tokens = np.array([0, vocab // 2, -1, vocab - 1])
+    nothing = np.full(4, -np.inf)
+    g, h = np.array([2.0, -0.5, 3.0, 0.0]), np.array([1.0, -4.0, 2.0, 0.25])
+    got, _ = gradient(x, tokens, nothing, np.zeros(4), g, h, tag, wt)
+    want = np.zeros((4, vocab))
+    want[0, 0], want[1, vocab // 2] = 2.0, -0.5
+    assert np.array_equal(got, want)
+    # the forward pass gives the lse and entropy used here
+    import torch
+    lp, ent, lse = (room((4,), wt) for _ in range(3))
+    tok = torch.from_numpy(tokens).cuda()
+    torch.cuda.synchronize()
+    eb.token_logprobs_device(x.data_ptr(), tok.data_ptr(), lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), 0, 0, 4, vocab, 0, tag)
+    done()
+    assert np.array_equal(wide64(lse), nothing) and np.array_equal(wide64(ent), np.zeros(4))
+    assert np.array_equal(wide64(lp), [-np.inf, -np.inf, 0.0, -np.inf])
