@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
 #include <type_traits>
 
 namespace b200 {
@@ -339,6 +340,9 @@ class DeviceScope {
 // Scratch of one operator call (b200_scratch.cu).  Outside a capture: a grow-only block of the
 // library, ordered by the library's stream.  While the library's stream is captured: stream-ordered
 // allocation nodes, so every graph owns its scratch and two graphs never share any.
+// The order of the stream protects the block only if one call's launches follow one another, and the block
+// may be replaced by a larger one: from reserve() to the end of its call an OpScratch holds a lock, and
+// calls of other host threads that need scratch wait for it (a few launches long).
 class OpScratch {
  public:
   ~OpScratch() { release(); }
@@ -346,6 +350,7 @@ class OpScratch {
   int release();                                    // ends the use; -1 when the free node failed
 
  private:
+  std::unique_lock<std::mutex> hold_;  // until destruction, after the call's last launch
   void* captured_ = nullptr;
   cudaStream_t st_ = nullptr;
 };

@@ -6,12 +6,14 @@
 
 namespace b200 {
 namespace {
+std::mutex g_mu;  // guards the block, and the launches of the call that uses it
 uint8_t* g_block = nullptr;
 size_t g_bytes = 0;
 }  // namespace
 
 uint8_t* OpScratch::reserve(size_t bytes, cudaStream_t st) {
   if (bytes == 0) bytes = 16;
+  hold_ = std::unique_lock<std::mutex>(g_mu);
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(st, &status) != cudaSuccess || status == cudaStreamCaptureStatusInvalidated) {
     fprintf(stderr, "[eshkol-b200] the library stream cannot be used: %s\n", cudaGetErrorString(cudaGetLastError()));
@@ -59,9 +61,13 @@ int OpScratch::release() {
   return 0;
 }
 
-size_t op_scratch_bytes() { return g_bytes; }
+size_t op_scratch_bytes() {
+  const std::lock_guard<std::mutex> lock(g_mu);
+  return g_bytes;
+}
 
 void op_scratch_shutdown() {
+  const std::lock_guard<std::mutex> lock(g_mu);
   if (g_block) cudaFree(g_block);
   g_block = nullptr;
   g_bytes = 0;

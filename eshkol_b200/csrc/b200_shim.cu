@@ -12,6 +12,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -32,7 +33,6 @@ struct State {
   uint8_t* ws = nullptr;
   size_t ws_bytes = 0;
   int* d_status = nullptr;
-  unsigned long long launches = 0;
   unsigned long long h2d_bytes = 0, d2h_bytes = 0;  // host <-> device bytes this library has moved
   cudaEvent_t ev_g0 = nullptr, ev_g1 = nullptr;     // around the last eshkol_b200_gemm_f64_device
   bool ev_g_valid = false;
@@ -111,6 +111,7 @@ struct State {
 };
 static State g;
 static std::mutex g_mu;
+static std::atomic<unsigned long long> g_launches{0};  // operator calls of several host threads count here
 
 #define B200_CHECK(call)                                                              \
   do {                                                                                \
@@ -215,7 +216,7 @@ static inline int gemm_sms() {
 }
 int lib_num_sms() { return gemm_sms(); }
 int* lib_status_word() { return g.d_status; }
-void count_launches(int n) { g.launches += static_cast<unsigned long long>(n); }
+void count_launches(int n) { g_launches += static_cast<unsigned long long>(n); }
 
 // rows x inner_bytes int8 planes, `planes` of them `plane_stride` bytes apart,
 // tiled {128 bytes, box_rows, 1} with the 128-byte swizzle; out-of-range rows and
@@ -483,7 +484,7 @@ static int oz2_prepare_b(const double* dB, long long K, long long N, int bn, boo
   else B200_CHECK(launch_split_b(dB, P.sb, N, pb, P.consts, st, view));
   B200_MARK(2);
   if (timed) ++g.n_evb;
-  g.launches += 3;
+  g_launches += 3;
   if (oz2_b_maps(q, bn)) return -1;
   P.valid = true;
   ++g.prep_token;
@@ -521,7 +522,7 @@ static int oz2_prepare_b_columns(const double* dB, long long ldb, long long K, l
   B200_CHECK(launch_split_b(dB, sb, ncols, pb, hc, st, nullptr, ldb));
   B200_MARK(2);
   if (timed) ++g.n_evb;
-  g.launches += 3;
+  g_launches += 3;
   return 0;
 }
 
@@ -582,7 +583,7 @@ static int oz2_prepare_a_at(State::PreparedA& A, uint8_t* ws, const Oz2Geom& q, 
   if (trans) B200_CHECK(launch_split_b(dA, A.sa, M, pa, hc, st));
   else B200_CHECK(launch_split_a(dA, A.sa, pa, hc, st));
   if (tev) B200_CHECK(cudaEventRecord(tev[2], st));
-  g.launches += 3;
+  g_launches += 3;
   if (make_plane_map(&A.mA0, A.a0, q.K0, M, 1, static_cast<long long>(M) * q.K0, kBM)) return -1;
   if (make_plane_map(&A.mA1, A.aodd, q.Kp, M, n_odd, A.a_stride, kBM)) return -1;
   A.valid = true;
@@ -720,7 +721,7 @@ static int oz2_multiply_at(const State::PreparedA& A, uint8_t* ws, size_t cap, d
   if (tev) B200_CHECK(cudaEventRecord(tev[5], sp));
   B200_CHECK(launch_crt(ca, P.consts, sp));
   if (tev) B200_CHECK(cudaEventRecord(tev[6], sp));
-  g.launches += 4;
+  g_launches += 4;
 
   State::Last& L = g.last;
   L.valid = true; L.M = M; L.K = P.K; L.N = P.N; L.Kp = A.Kp; L.K0 = A.K0; L.Mp = A.Mp; L.Np = P.Np;
@@ -973,7 +974,7 @@ static int ozaki2_gemm_general(const double* dA, const double* dB, double* dC, l
   ca.activation = o.activation;
   ca.pixels_per_image = o.pixels_per_image;
   B200_CHECK(launch_crt(ca, hc, st));
-  g.launches += 10;
+  g_launches += 10;
 
   State::Last& L = g.last;
   L.valid = true; L.M = M; L.K = K; L.N = N; L.Kp = q.Kp; L.K0 = q.K0; L.Mp = q.Mp; L.Np = q.Np;
@@ -1265,6 +1266,7 @@ void eshkol_b200_shutdown(void) {
   }
   cudaStreamDestroy(g.stream);
   g = State();
+  g_launches = 0;
 }
 
 void* eshkol_b200_stream(void) { return g.ready ? static_cast<void*>(g.stream) : nullptr; }
@@ -1296,7 +1298,7 @@ int eshkol_b200_gemm_f64_device(const double* dA, const double* dB, double* dC, 
       B200_CHECK(launch_transpose(dB, n, k, reinterpret_cast<double*>(t + ba), g.stream));
       dB = reinterpret_cast<const double*>(t + ba);
     }
-    g.launches += (o.trans_a ? 1 : 0) + (o.trans_b ? 1 : 0);
+    g_launches += (o.trans_a ? 1 : 0) + (o.trans_b ? 1 : 0);
     o.trans_a = o.trans_b = 0;
   }
   g.ev_g_valid = false;
@@ -1607,7 +1609,7 @@ int eshkol_b200_elementwise_f64_device(const double* a, const double* b, double*
                                        uint64_t n, int op) {
   if (!g.ready || !a || !out || n == 0 || op < 0 || op > 14) return -1;
   B200_CHECK(launch_elementwise(a, b, out, static_cast<long long>(n), op, g.stream));
-  g.launches += 1;
+  g_launches += 1;
   return 0;
 }
 
@@ -1843,7 +1845,7 @@ void eshkol_b200_debug_set_wait_limit_ns(unsigned long long ns) { g_dbg_wait_ns 
 void eshkol_b200_debug_fail_allocation(int nth) { g_dbg_fail_alloc = nth > 0 ? nth : 0; }
 void eshkol_b200_debug_withhold_arrival(int on) { g_dbg_withhold = on ? 1 : 0; }
 
-uint64_t eshkol_b200_launch_count(void) { return g.launches; }
+uint64_t eshkol_b200_launch_count(void) { return g_launches; }
 uint64_t eshkol_b200_workspace_bytes(void) { return g.ws_bytes + g.aux_bytes + g.bside_bytes + op_scratch_bytes(); }
 
 int eshkol_b200_debug_fetch(int what, int index, void* host_dst, uint64_t capacity_bytes,

@@ -11,6 +11,10 @@
  * All functions use plain C types.  Unless stated otherwise they return 0 on
  * success and a negative value on failure, and they enqueue work on the
  * library's stream without waiting for it.
+ *
+ * Host threads: the operators of training and serving may be called by several
+ * host threads at once.  Everything else works in one workspace and belongs to
+ * one host thread at a time.
  */
 #ifndef ESHKOL_B200_EXT_H
 #define ESHKOL_B200_EXT_H
@@ -294,7 +298,8 @@ int eshkol_b200_layernorm_backward_f64_device(const double* grad_out, const doub
  * nothing (sums over them are zero).  Statistics and the gradients of vectors are f64 for f64 tensors and
  * f32 otherwise ("stat type"); sums are held in that type and combined in a fixed order, so equal calls
  * give equal bits.  Arrays must not overlap unless the call says so.
- * Scratch belongs to the library and is ordered by its stream.  Calls captured from that stream into a
+ * Scratch belongs to the library and is ordered by its stream; calls of several host threads are enqueued one
+ * after the other where they need it.  Calls captured from that stream into a
  * CUDA graph get scratch of the graph's own, so graphs may be replayed on any stream and beside eager
  * calls; a replay itself is ordered by the stream it is launched on. */
 typedef enum {
