@@ -1135,11 +1135,10 @@ int linear_gradients(const LinearArgs& a, const void* grad_out, void* grad_x, vo
     if (!grad_w && !grad_bias) return launches;
   }
   const bool products = grad_x || grad_w;
-  Carver cv;
+  Carver cv, none;  // an operand that no product reads takes no scratch
   // dz: grad_out itself when there is no activation and the products can read it
-  Operand<T> dz(grad_out, a.rows, a.d_out, a.ldy, a.o.activation != 0, cv);
-  Operand<T> x(a.x, a.rows, a.d_in, a.ldx, false, cv);
-  Carver none;  // an operand that no product reads takes no scratch
+  Operand<T> dz(grad_out, a.rows, a.d_out, a.ldy, a.o.activation != 0, products ? cv : none);
+  Operand<T> x(a.x, a.rows, a.d_in, a.ldx, false, grad_w ? cv : none);
   Operand<T> w(a.w, tw ? a.d_out : a.d_in, tw ? a.d_in : a.d_out, a.ldw, false, grad_x ? cv : none);
   ProductSpec s[2];
   LinProduct epi[2];

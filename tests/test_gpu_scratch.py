@@ -72,3 +72,49 @@ def test_two_host_threads(gpu_lib):
         done()
         for (_, outs), w in zip(mine + others, want):
             assert all(np.array_equal(wide64(o), v) for o, v in zip(outs, w))
+
+
+SCRATCH_PROGRAM = """
+import sys
+import torch
+import eshkol_b200 as eb
+lib = eb.load_library()
+assert lib.eshkol_gpu_init() == 1
+rows, k, n = 2000, 3000, 5000
+kinds = {"f32": (torch.float32, eb.DTYPE_F32), "f16": (torch.float16, eb.DTYPE_F16)}
+t, tag = kinds[sys.argv[1]]
+x, w, g, z = (torch.zeros(a, b + 1, dtype=t, device="cuda")[:, :b] for a, b in ((rows, k), (k, n), (rows, n), (rows, n)))
+gb = torch.empty(n, device="cuda")
+torch.cuda.synchronize()
+P = lambda v: v.data_ptr() if v is not None else 0
+opts = eb.make_linear_opts(tag, activation=2, pre=P(z), ldx=k + 1, ldw=n + 1, ldy=n + 1, ld_pre=n + 1)
+for wanted in ("b", "x", "w"):
+    ox = torch.zeros(rows, k + 1, dtype=t, device="cuda")
+    ow = torch.zeros(k, n + 1, dtype=t, device="cuda")
+    torch.cuda.synchronize()
+    eb.linear_gradients_device(P(g), P(x) if wanted == "w" else 0, P(w) if wanted == "x" else 0, P(ox) if wanted == "x" else 0,
+                               P(ow) if wanted == "w" else 0, P(gb) if wanted == "b" else 0, rows, k, n, opts)
+    assert eb.sync_status() == 0
+    print(wanted, lib.eshkol_b200_workspace_bytes())
+"""
+
+
+@pytest.mark.parametrize("dtype,planes", [("f32", 3), ("f16", 1)])
+def test_only_operands_of_a_product_take_scratch(gpu_lib, dtype, planes):
+    """In a process of its own, whose scratch has not grown yet: the bias' gradient alone needs its partial
+    sums, the gradient of x no copy of x, that of w no copy of w (partial sums of a split reduction aside)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", SCRATCH_PROGRAM, dtype], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
+    held = {line.split()[0]: int(line.split()[1]) for line in run.stdout.splitlines()}
+    rows, k, n = 2000, 3000, 5000
+    pad = lambda c: (c + 7) // 8 * 8  # noqa: E731
+    dz, x, w = rows * pad(n) * 2 * planes, rows * pad(k) * 2 * planes, k * pad(n) * 2 * planes
+    # partial sums of at most 512 groups of rows: 20 blocks across, and no more in all than the SMs hold
+    assert held["b"] <= 512 * n * 4 + 4096, held
+    # room for rounding every part up to 1024 bytes; at these sizes no reduction is split
+    assert held["x"] <= dz + w + 8192, held
+    assert held["w"] <= max(dz + x, dz + w) + 8192, held
