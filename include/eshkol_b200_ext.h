@@ -330,8 +330,10 @@ int eshkol_b200_layernorm_gradients_device(const void* grad_out, const void* x, 
  *   y = activation(z) + residual
  * x [rows x d_in], w [d_in x d_out] (with trans_w [d_out x d_in]), bias [d_out], residual, y and pre
  * [rows x d_out], all in opts->dtype.  16-bit operands are multiplied on the tensor cores as they lie
- * (rows that are not on 16-byte boundaries are copied to scratch first) with f32 sums; f32 operands as
- * three bf16 parts each, exact to f32 rounding for finite values below 3.38e38 (others give NaN).  f64
+ * (rows that are not on 16-byte boundaries are copied to scratch first) with f32 sums.  f32 operands are
+ * multiplied as three bf16 parts each, products exact to f32 rounding for zeros and magnitudes from 2^-103 to
+ * 3.38e38; smaller numbers lose what is below 2^-125, larger ones and infinities make results NaN.  With up
+ * to 16 rows y and grad_x are made from f32 operands as they are (12 where w is stored along the reduction).  f64
  * tensors are refused: eshkol_b200_gemm_f64_device and _feed_forward_f64_device serve them. */
 typedef struct EshkolB200LinearOpts {
   int32_t dtype;            /* EshkolB200Dtype: F32, F16 or BF16 */

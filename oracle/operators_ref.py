@@ -181,3 +181,26 @@ def linear_gradients(g, x, w, pre, act):
     """(grad_x, grad_w, grad_bias, dz)."""
     dz = g * activate_slope(pre, act) if act else g
     return dz @ w.T, x.T @ dz, dz.sum(axis=0), dz
+
+
+# ---- f32 products by bf16 parts, as the linear layer multiplies them
+def to_bf16(x):
+    """f32 values rounded to the nearest bf16 (ties to even), as f32; finite input"""
+    b = np.asarray(x, dtype=np.float32).view(np.uint32)
+    b = (b + np.uint32(0x7FFF) + ((b >> np.uint32(16)) & np.uint32(1))) & np.uint32(0xFFFF0000)
+    return b.view(np.float32)
+
+
+def bf16_parts(x, count=3):
+    """The leading `count` parts of f32 values; three of them add up to the value."""
+    rest, parts = np.asarray(x, dtype=np.float32), []
+    for _ in range(count):
+        parts.append(to_bf16(rest))
+        rest = (rest - parts[-1]).astype(np.float32)
+    return parts
+
+
+def product_of_parts(x, w, count=3):
+    """x @ w in f64 from the products of parts i, j with i + j < count (six of nine for three parts)"""
+    a, b = ([p.astype(np.float64) for p in bf16_parts(v, count)] for v in (x, w))
+    return sum(a[i] @ b[j] for i in range(count) for j in range(count - i))
