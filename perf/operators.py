@@ -267,8 +267,22 @@ def _ptr(t):
 
 
 def _own(s):
+    """The calls, which run on the library's stream: it waits for torch's stream, which has written a new state,
+    and torch's stream waits for the results of every pass."""
     import eshkol_b200 as eb
 
+    torchs = torch.cuda.current_stream()
+    if "library" not in s:
+        eb.load_library().eshkol_gpu_init()
+        s["library"], s["results"] = torch.cuda.ExternalStream(eb.stream_handle()), torch.cuda.Event()
+        s["library"].wait_stream(torchs)
+    out = _calls(s, eb)
+    s["results"].record(s["library"])
+    torchs.wait_event(s["results"])
+    return out
+
+
+def _calls(s, eb):
     dtype = {torch.float64: eb.DTYPE_F64, torch.float32: eb.DTYPE_F32, torch.float16: eb.DTYPE_F16, torch.bfloat16: eb.DTYPE_BF16}[s["torch_dtype"]]
     op = s["op"]
     if op == "norm":
