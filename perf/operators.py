@@ -267,19 +267,17 @@ def _ptr(t):
 
 
 def _own(s):
-    """The calls, which run on the library's stream: it waits for torch's stream, which has written a new state,
-    and torch's stream waits for the results of every pass."""
+    """The calls, on the library's stream, where the program's torch work moves with its first call: what torch has
+    written comes before them, what it does with the results behind them."""
     import eshkol_b200 as eb
 
-    torchs = torch.cuda.current_stream()
-    if "library" not in s:
+    if "moved" not in s:
         eb.load_library().eshkol_gpu_init()
-        s["library"], s["results"] = torch.cuda.ExternalStream(eb.stream_handle()), torch.cuda.Event()
-        s["library"].wait_stream(torchs)
-    out = _calls(s, eb)
-    s["results"].record(s["library"])
-    torchs.wait_event(s["results"])
-    return out
+        library = torch.cuda.ExternalStream(eb.stream_handle())
+        library.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(library)
+        s["moved"] = True
+    return _calls(s, eb)
 
 
 def _calls(s, eb):
