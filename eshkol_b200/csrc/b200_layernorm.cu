@@ -24,15 +24,17 @@ namespace b200 {
 namespace {
 namespace cg = cooperative_groups;
 
-// What the deviations are taken from: the row's first mean, rounded to the tensor's own type.  For 16-bit
-// tensors differences from it are exact (of numbers up to 2^13 times it) and share no rounding, which those
-// from an f32 mean do; and no entry is nearer to the mean than the nearest number of the type, so off^2, which
-// the correction takes from the mean square, is at most half of it.  For f32 and f64 tensors it is the mean
-// itself, off by its sum's rounding alone.  Measured: f32 rows with a mean of 10^6 deviations are right to 7e-7
-// and f64 rows at 10^10 to 1e-15 (from a pivot of ten bits 2e-3 and 4e-4).
-template <typename T> __device__ __forceinline__ typename Elem<T>::Acc pivot_of(typename Elem<T>::Acc mean) {
-  return Elem<T>::widen(Elem<T>::narrow(mean));
+// What the deviations are taken from, the pivot: the first places of the mean, at least 10 bits of it.  x minus
+// it is exact for x up to 2^13 times it; from the whole mean all x of one binade would share a rounding, and
+// with it the correction by the deviations' own sum (rows around zero: their mean off by 10^-6 instead of 10^-7).
+// Where the mean is more than some 10^3 deviations the correction is larger than these, and taking its square from
+// the mean square would cancel: such a row (off_too_far) takes its deviations once more, from the corrected mean,
+// which they are so close to that the differences are exact again.
+__device__ __forceinline__ float leading_bits(float v) { return __uint_as_float(__float_as_uint(v) & 0xffffe000u); }
+__device__ __forceinline__ double leading_bits(double v) {
+  return __longlong_as_double(__double_as_longlong(v) & ~0x3ffffffffffll);
 }
+template <typename A> __device__ __forceinline__ bool off_too_far(A off, A var) { return off * off > var; }
 
 struct NormArgs {
   const void *x, *gamma, *beta;
@@ -57,8 +59,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 25
   using D = Duo<A>;
   constexpr int kV = kVec16<T>, kD = kDuos<T>, kAhead = kNormAhead<kThreads, kHow>;
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ A sm1[32], sm2[64];
+  __shared__ A sm1[32], sm2[64], sm3[64];
   constexpr int width = kWarp ? 32 : kThreads, warps = kWarp ? 1 : kThreads / 32, per_block = kWarp ? kThreads / 32 : 1;
+  constexpr int kWritten = sizeof(T) == 8 ? 2 : 1;
   const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, group = kWarp ? threadIdx.x >> 5 : 0;
   const int n = a.n;
   const T *gamma = static_cast<const T*>(a.gamma), *beta = static_cast<const T*>(a.beta);
@@ -111,35 +114,45 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 25
       for (int j = 0; j < kD; ++j) sum2[j] = sum2[j] + d[i][j];  // places behind the row hold zero
 #pragma unroll
     for (int j = 1; j < kD; ++j) sum2[0] = sum2[0] + sum2[j];
-    const A pivot = pivot_of<T>(block_sum(total(sum2[0]), sm1, warps) * inv_n);
-    D ds2[kD], sq2[kD];
+    const A pivot = leading_bits(block_sum(total(sum2[0]), sm1, warps) * inv_n);
+    A off, var, mean = A(0), by = pivot;
+    // Once, or twice; the same for the whole row.  Written out twice for f64 alone: 60000 x 500 takes 100 us so
+    // and 104 as a loop, but 8192 x 4096 bf16 in pairs 64 so, 53 as a loop (and 59 without a second time).
+#pragma unroll kWritten
+    for (A* sm = sm2;; sm = sm3) {
+      D ds2[kD], sq2[kD];
 #pragma unroll
-    for (int j = 0; j < kD; ++j) ds2[j] = sq2[j] = both(A(0));
+      for (int j = 0; j < kD; ++j) ds2[j] = sq2[j] = both(A(0));
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int c = (t + i * width) * kV;
-      if (c >= n) break;
+      for (int i = 0; i < kN; ++i) {
+        const int c = (t + i * width) * kV;
+        if (c >= n) break;
 #pragma unroll
-      for (int j = 0; j < kD; ++j) {
-        d[i][j] = d[i][j] + both(-pivot);
-        if constexpr (kHow != kByWords)  // the row may end inside a word: what is behind it deviates by nothing
-          d[i][j] = D::of(c + 2 * j < n ? d[i][j].lo() : A(0), c + 2 * j + 1 < n ? d[i][j].hi() : A(0));
-        ds2[j] = ds2[j] + d[i][j];
-        sq2[j] = fma2(d[i][j], d[i][j], sq2[j]);
+        for (int j = 0; j < kD; ++j) {
+          d[i][j] = d[i][j] + both(-by);
+          if constexpr (kHow != kByWords)  // the row may end inside a word: what is behind it deviates by nothing
+            d[i][j] = D::of(c + 2 * j < n ? d[i][j].lo() : A(0), c + 2 * j + 1 < n ? d[i][j].hi() : A(0));
+          ds2[j] = ds2[j] + d[i][j];
+          sq2[j] = fma2(d[i][j], d[i][j], sq2[j]);
+        }
       }
-    }
 #pragma unroll
-    for (int j = 1; j < kD; ++j) {
-      ds2[0] = ds2[0] + ds2[j];
-      sq2[0] = sq2[0] + sq2[j];
+      for (int j = 1; j < kD; ++j) {
+        ds2[0] = ds2[0] + ds2[j];
+        sq2[0] = sq2[0] + sq2[j];
+      }
+      A ds = total(ds2[0]), sq = total(sq2[0]);
+      block_sum2(ds, sq, sm, warps);
+      off = ds * inv_n;
+      var = sq * inv_n - off * off;
+      mean += by;
+      if (sm == sm3 || !off_too_far(off, var)) break;
+      by = off;
     }
-    A ds = total(ds2[0]), sq = total(sq2[0]);
-    block_sum2(ds, sq, sm2, warps);
-    const A off = ds * inv_n;  // mean = pivot + off
-    const A var = sq * inv_n - off * off;
+    mean += off;
     const A r_std = inverse_root((var > A(0) ? var : var * A(0)) + epsilon);  // a NaN stays one
     if (t == 0) {
-      if (a.mean) static_cast<A*>(a.mean)[r] = pivot + off;
+      if (a.mean) static_cast<A*>(a.mean)[r] = mean;
       if (a.inv_std) static_cast<A*>(a.inv_std)[r] = r_std;
     }
 #pragma unroll
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(
     typename Elem<T>::Acc* __restrict__ mean_out, typename Elem<T>::Acc* __restrict__ inv_std_out, long long rows,
     int n, long long ldx, long long ldy, typename Elem<T>::Acc epsilon) {
   using A = typename Elem<T>::Acc;
-  __shared__ A sm1[32], sm[64];
+  __shared__ A sm1[32], sm2[64], sm3[64];
   const int warps = blockDim.x >> 5;
   const A inv_n = A(1) / A(n);
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -176,25 +189,40 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(
     T* out = y + r * ldy;
     A sum = 0;
     for (int c = threadIdx.x; c < n; c += blockDim.x) sum += Elem<T>::widen(in[c]);
-    const A mean0 = pivot_of<T>(block_sum(sum, sm1, warps) * inv_n);
-    A ds = 0, sq = 0;
-    for (int c = threadIdx.x; c < n; c += blockDim.x) {
-      const A d = Elem<T>::widen(in[c]) - mean0;
-      ds += d;
-      sq += d * d;
+    const A mean0 = leading_bits(block_sum(sum, sm1, warps) * inv_n);
+    const auto deviations = [&](A more, A& ds, A& sq, A* sm) {
+      ds = sq = 0;
+      for (int c = threadIdx.x; c < n; c += blockDim.x) {
+        const A d = (Elem<T>::widen(in[c]) - mean0) - more;
+        ds += d;
+        sq += d * d;
+      }
+      block_sum2(ds, sq, sm, warps);
+    };
+    A ds, sq, far = 0;  // far: from the pivot to where the deviations are taken from
+    deviations(far, ds, sq, sm2);
+    A off = ds * inv_n, mean = mean0 + off;
+    A var = sq * inv_n - off * off;
+    if (off_too_far(off, var)) {  // the same for the whole row
+      far = off;
+      deviations(far, ds, sq, sm3);
+      off = ds * inv_n;
+      mean += off;
+      var = sq * inv_n - off * off;
     }
-    block_sum2(ds, sq, sm, warps);
-    const A off = ds * inv_n;
-    const A var = sq * inv_n - off * off;
     const A r_std = inverse_root((var > A(0) ? var : var * A(0)) + epsilon);
     if (threadIdx.x == 0) {
-      if (mean_out) mean_out[r] = mean0 + off;
+      if (mean_out) mean_out[r] = mean;
       if (inv_std_out) inv_std_out[r] = r_std;
     }
-    for (int c = threadIdx.x; c < n; c += blockDim.x) {
-      const A xhat = ((Elem<T>::widen(in[c]) - mean0) - off) * r_std;
-      out[c] = Elem<T>::narrow(xhat * (gamma ? Elem<T>::widen(gamma[c]) : A(1)) + (beta ? Elem<T>::widen(beta[c]) : A(0)));
-    }
+    const auto results = [&](auto centred) {
+      for (int c = threadIdx.x; c < n; c += blockDim.x) {
+        const A xhat = centred(Elem<T>::widen(in[c])) * r_std;
+        out[c] = Elem<T>::narrow(xhat * (gamma ? Elem<T>::widen(gamma[c]) : A(1)) + (beta ? Elem<T>::widen(beta[c]) : A(0)));
+      }
+    };
+    if (far == A(0)) results([&](A v) { return (v - mean0) - off; });
+    else results([&](A v) { return ((v - mean0) - far) - off; });
   }
 }
 

@@ -88,3 +88,17 @@ def test_constant_rows_have_no_deviation(gpu_lib, dtype):
     assert np.all(np.abs(mean - level) <= 3 * u * np.abs(level))
     # a deviation is the difference of the first mean's error and its correction
     assert np.all(np.abs(y).max(axis=1) <= 36 * u * (34 * u * np.abs(level)) * wi * 2 + 1e-12)
+
+
+@pytest.mark.parametrize("rows,n", [(2000, 4096), (100, 2001), (20, 20000)])
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+def test_means_near_zero(gpu_lib, dtype, rows, n):
+    """Means of a fiftieth of the deviations.  The sum of the deviations reaches sqrt(n) and its last levels of
+    additions leave about 2 * 2^-1 u sqrt(n) of it, sqrt(1 / n) u per entry or 50 / sqrt(n) u of the mean,
+    whose own rounding is another half u: 1.6 u at n = 1000, in norm over the rows, and 4 u are allowed.
+    Differences that share a rounding, half a step of u on average a quarter, would leave 12 u."""
+    t, tag, wt, u, half = kinds(dtype)
+    x = laid(inputs.normal(132, (rows, n)) + 0.02, t)
+    y, mean, inv = forward(x, rows, n, tag, wt, 0.0)
+    want, wm, wi = definition(wide64(x), 0.0)
+    assert np.linalg.norm((mean - wm).astype(np.float64)) <= 4 * u * np.linalg.norm(wm.astype(np.float64))
