@@ -248,8 +248,8 @@ template <int kLeft> __device__ __forceinline__ void wait_async() {
 }
 
 // Launches of one operator that follow one another (launch_after): the next kernel's blocks may come to the
-// SMs as soon as all blocks of the one before have called let_next_start, and wait in after_previous, their
-// first instruction, until that kernel is complete and its writes are visible.  That hides the start of the
+// SMs as soon as all blocks of the one before have called let_next_start, and wait in after_previous, before
+// they touch global memory, until that kernel is complete and its writes are visible.  That hides the start of the
 // launch, 1 to 2 us.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -47,8 +47,8 @@ struct NormArgs {
 
 // ------------------------------------------------------------------ forward
 // A row belongs to a warp, or to a block, whose threads hold kN words of 16 bytes each.  What a thread does
-// once per row (its share of the reductions, the root, addresses) is some 150 instructions, an element
-// about ten (packed f32 arithmetic), so a thread gets four words where rows are many.  The next kAhead
+// once per row (its share of the reductions, the root, addresses) is some 150 instructions, an element of a
+// bf16 row 20 in all (packed f32 arithmetic), so a thread gets four words where rows are many.  The next kAhead
 // rows are on their way in shared memory: every thread copies the words that it will read itself.  Measured at
 // 8192 x 4096 bf16: 128 threads with four words 39 us, 64 with eight 46, a warp with sixteen 53.
 template <int kThreads, int kHow> constexpr int kNormAhead = kHow == kInRegisters ? 1 : kThreads == 1024 ? 2 : 4;
@@ -238,9 +238,10 @@ struct NormGradArgs {
 // A row belongs to a warp, to a block, or to the blocks of a cluster, each with a contiguous part of the
 // columns.  A thread keeps its columns (kN words of 16 bytes) over all rows of its group, and with them
 // its share of grad_gamma and grad_beta in registers; a block's share goes to partial[group][2][n].  Many
-// elements a thread and few warps a row, because what a thread does once per row costs as much as ten elements.  The next rows are on their way in shared memory, kAhead of them (every thread
-// copies the words that it will read itself, so no barrier is involved), or, where the rows are not on
-// 16-byte boundaries, one in registers.
+// elements a thread and few warps a row, because what a thread does once per row costs as much as ten
+// elements.  The next rows are on their way in shared memory, kAhead of them (every thread copies the words
+// that it will read itself, so no barrier is involved), or, where the rows are not on 16-byte boundaries, one
+// in registers.
 // words a thread holds in a row of a block: 16 elements, or 8 of f64
 template <typename T> constexpr int kGradWords = sizeof(T) == 2 ? 2 : 4;
 template <int kN, int kHow> constexpr int kRowsAhead = kHow == kInRegisters ? 1 : 4;

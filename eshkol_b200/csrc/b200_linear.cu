@@ -5,7 +5,7 @@
 //   dz = grad_out act'(pre),  grad_x = dz W^T,  grad_w = x^T dz,  grad_b = sum over rows of dz
 //
 // One persistent kernel multiplies: warp 0 loads operand tiles by TMA into a ring of shared-memory
-// stages, warp 1 issues tcgen05.mma into one of two TMEM accumulators, warps 2-5 drain the other one.
+// stages, warp 1 issues tcgen05.mma into one of two TMEM accumulators, warps 2-9 drain the other one.
 // Each operand is read as it lies, with the reduction axis along its rows ("K-major") or across them
 // ("MN-major"): the matrix descriptors take both, so no product needs a transposed copy.  Sums are f32 in
 // TMEM; a result is rounded to the storage type once.
@@ -17,8 +17,8 @@
 // Bound by the tensor pipe (active 94 % of the time on pairs of SMs): 8192 x 16384 x 4096 bf16 takes 725 us in
 // a burst, 1517 TFLOP/s, and 850 under the power cap; all gradients at 4096 x 4096 x 16384 755 us in a burst.
 //
-// A few rows: b200_linear_small.cu.  Few output tiles and a long reduction: the reduction is split over blocks, their f32 sums go to scratch
-// and a second kernel adds them in order and applies the epilogue.
+// A few rows: b200_linear_small.cu.  Few output tiles and a long reduction: the reduction is split over
+// blocks, their f32 sums go to scratch and a second kernel adds them in order and applies the epilogue.
 #include <math.h>
 #include <stdio.h>
 #include <string.h>

@@ -15,8 +15,8 @@ struct LinEpilogue {
 };
 
 // ------------------------------------------------------------------ activations
-// Roundings are written out (no contraction left to the compiler), so that a result does not depend on
-// which other results a call asks for.
+// Roundings are written out (no contraction left to the compiler), so that a forward result does not depend
+// on which other results a call asks for.  (Which gradients are asked for decides how reductions are cut.)
 template <bool kExact> __device__ __forceinline__ float logistic(float v) {
   if (kExact) return __fdiv_rn(1.f, __fadd_rn(1.f, expf(-v)));
   // a few 2^-22: below half a step of the 16-bit results

@@ -347,7 +347,8 @@ typedef struct EshkolB200LinearOpts {
 } EshkolB200LinearOpts;
 int eshkol_b200_linear_forward_device(const void* x, const void* w, void* y, uint64_t rows, uint64_t d_in,
                                       uint64_t d_out, const EshkolB200LinearOpts* opts);
-/* Its gradients: with dz = grad_out * activation'(pre), which 16-bit tensors round once for the products,
+/* Its gradients: with dz = grad_out * activation'(pre), which 16-bit tensors round once for the products (grad_x
+ * of a few rows, 8 at most, is made from the unrounded dz),
  *   grad_x = dz w^T,  grad_w = x^T dz (stored as w is),  grad_bias = column sums of the unrounded dz
  * grad_out [rows x d_out] has the pitch ldy, grad_x that of x, grad_w that of w; grad_bias [d_out] is f32.
  * Each result may be NULL, not all of them; x may be NULL without grad_w, w without grad_x.  opts->bias
@@ -358,7 +359,7 @@ int eshkol_b200_linear_gradients_device(const void* grad_out, const void* x, con
 
 /* Log probabilities of given tokens under rows of logits [rows x vocab], vocab <= 2^30, rows <= 2^24:
  *   lse = log sum exp(logits),  logprob = logits[token] - lse,  entropy = -sum p log p
- * and the n_top <= 32 largest logits of every row: their log probabilities [rows x n_top] and indices,
+ * and the n_top <= 32 (and <= vocab) largest logits of every row: their log probabilities [rows x n_top] and indices,
  * largest first, equal logits by index.  tokens [rows]; a negative token stands for a position without
  * one (logprob 0), a token >= vocab gives NaN.  logprob, entropy, lse, top_logprob are in the stat type;
  * each output may be NULL, not all of them; n_top is 0 exactly when both top outputs are NULL; tokens may
