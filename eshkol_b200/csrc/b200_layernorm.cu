@@ -48,7 +48,7 @@ struct NormArgs {
 // ------------------------------------------------------------------ forward
 // A row belongs to a warp, or to a block, whose threads hold kN words of 16 bytes each.  What a thread does
 // once per row (its share of the reductions, the root, addresses) is some 150 instructions, an element of a
-// bf16 row 20 in all (packed f32 arithmetic), so a thread gets four words where rows are many.  The next kAhead
+// bf16 row 21 in all (packed f32 arithmetic), so a thread gets four words where rows are many.  The next kAhead
 // rows are on their way in shared memory: every thread copies the words that it will read itself.  Measured at
 // 8192 x 4096 bf16: 128 threads with four words 39 us, 64 with eight 46, a warp with sixteen 53.
 template <int kThreads, int kHow> constexpr int kNormAhead = kHow == kInRegisters ? 1 : kThreads == 1024 ? 2 : 4;
