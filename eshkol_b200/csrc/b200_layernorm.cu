@@ -35,6 +35,12 @@ __device__ __forceinline__ double leading_bits(double v) {
   return __longlong_as_double(__double_as_longlong(v) & ~0x3ffffffffffll);
 }
 template <typename A> __device__ __forceinline__ bool off_too_far(A off, A var) { return off * off > var; }
+// The mean itself is the pivot and the correction, except where it is far below the deviations: the first sum,
+// of entries of few bits, is then the more exact one (18000 f16 entries, mean of 2^-8 deviations: 10^-7 of the
+// mean against 10^-6).
+template <typename A> __device__ __forceinline__ A better_mean(A first, A corrected, A var) {
+  return first * first * A(256) < var ? first : corrected;
+}
 
 struct NormArgs {
   const void *x, *gamma, *beta;
@@ -114,8 +120,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 25
       for (int j = 0; j < kD; ++j) sum2[j] = sum2[j] + d[i][j];  // places behind the row hold zero
 #pragma unroll
     for (int j = 1; j < kD; ++j) sum2[0] = sum2[0] + sum2[j];
-    const A pivot = leading_bits(block_sum(total(sum2[0]), sm1, warps) * inv_n);
-    A off, var, mean = A(0), by = pivot;
+    const A first_mean = block_sum(total(sum2[0]), sm1, warps) * inv_n;
+    A off, var, mean = A(0), by = leading_bits(first_mean);
     // Once, or twice; the same for the whole row.  Written out twice for f64 alone: 60000 x 500 takes 100 us so
     // and 104 as a loop, but 8192 x 4096 bf16 in pairs 64 so, 53 as a loop (and 59 without a second time).
 #pragma unroll kWritten
@@ -149,10 +155,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : kThreads == 25
       if (sm == sm3 || !off_too_far(off, var)) break;
       by = off;
     }
-    mean += off;
     const A r_std = inverse_root((var > A(0) ? var : var * A(0)) + epsilon);  // a NaN stays one
     if (t == 0) {
-      if (a.mean) static_cast<A*>(a.mean)[r] = mean;
+      if (a.mean) static_cast<A*>(a.mean)[r] = better_mean(first_mean, mean + off, var);
       if (a.inv_std) static_cast<A*>(a.inv_std)[r] = r_std;
     }
 #pragma unroll
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(
     T* out = y + r * ldy;
     A sum = 0;
     for (int c = threadIdx.x; c < n; c += blockDim.x) sum += Elem<T>::widen(in[c]);
-    const A mean0 = leading_bits(block_sum(sum, sm1, warps) * inv_n);
+    const A first_mean = block_sum(sum, sm1, warps) * inv_n, mean0 = leading_bits(first_mean);
     const auto deviations = [&](A more, A& ds, A& sq, A* sm) {
       ds = sq = 0;
       for (int c = threadIdx.x; c < n; c += blockDim.x) {
@@ -212,7 +217,7 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(
     }
     const A r_std = inverse_root((var > A(0) ? var : var * A(0)) + epsilon);
     if (threadIdx.x == 0) {
-      if (mean_out) mean_out[r] = mean;
+      if (mean_out) mean_out[r] = better_mean(first_mean, mean, var);
       if (inv_std_out) inv_std_out[r] = r_std;
     }
     const auto results = [&](auto centred) {

@@ -102,3 +102,16 @@ def test_means_near_zero(gpu_lib, dtype, rows, n):
     y, mean, inv = forward(x, rows, n, tag, wt, 0.0)
     want, wm, wi = definition(wide64(x), 0.0)
     assert np.linalg.norm((mean - wm).astype(np.float64)) <= 4 * u * np.linalg.norm(wm.astype(np.float64))
+
+
+@pytest.mark.parametrize("rows,n", [(40, 18000), (600, 16000), (100, 70000), (700, 6000)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_means_near_zero_of_16_bits(gpu_lib, dtype, rows, n):
+    """Wide rows with means of a hundredth of the deviations.  Sums of 16-bit entries keep their 8 or 11 bits
+    and the few of the count, so the first additions are exact and the last leave u sqrt(n) at most: with the
+    mean's own rounding 100 / sqrt(n) + 1.5 u of the mean, 3 u in norm, and 4 u are allowed."""
+    t, tag, wt, u, half = kinds(dtype)
+    x = laid(2.0 * inputs.normal(133, (rows, n)) + 0.02, t)
+    y, mean, inv = forward(x, rows, n, tag, wt, 0.0)
+    want, wm, wi = definition(wide64(x), 0.0)
+    assert np.linalg.norm((mean - wm).astype(np.float64)) <= 4 * u * np.linalg.norm(wm.astype(np.float64))
